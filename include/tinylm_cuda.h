@@ -228,6 +228,72 @@ int tl_model_step_zero1(void *handle, float *P, float *G, float *M_shard, float 
                         const int *tgt, const int *tgt_mtp, int B, float lr, int t, float max_norm,
                         float *loss_dev, float *norm_dev);
 
+/* ------------------------------------------- vocabulary rows (logits) */
+/* Operators over rows of logits: N rows of V values, row n at logits + n*ld
+ * elements (ld >= V, any alignment of the element type), of `dtype` TL_F32,
+ * TL_BF16 or TL_F16.  N >= 0 (0: nothing is done), 1 <= V <= TL_VOCAB_MAX,
+ * 1e-6 <= temperature <= 1e6.  With y = z/temperature:
+ *   log p_v = y_v - log sum_u exp(y_u),   H = -sum_v p_v log p_v.
+ * Sums, statistics and every float output are fp32 whatever the logits' type.
+ * A logit of -inf is a token of probability 0.  A row of -inf only has
+ * log p = -inf, H = 0 and no gradient; a type's lowest finite value is an
+ * ordinary logit (a row of it is uniform).  A row holding a NaN or +inf has no
+ * distribution: its results are NaN (top_ids -1).
+ * Token ids are device int32.  -1 is "none"; any other id outside [0, V) is
+ * taken as -1 and makes the next tl_device_status() return TL_EINVAL.
+ * The calls take no workspace, so they can be captured into CUDA graphs. */
+#define TL_F32  0
+#define TL_BF16 1
+#define TL_F16  2
+#define TL_TOPK_MAX  128
+#define TL_VOCAB_MAX 262144
+/* Scores rows of logits.  Each output may be NULL:
+ *   logp[n]     log p of ids[n] (ids and logp come together); 0 where ids[n] is -1
+ *   entropy[n]  H
+ *   stats[n][2] {largest logit, log of the sum of exp((z - largest)/temperature)},
+ *               what the gradient below needs
+ *   top_ids[n][K], top_logp[n][K]  the K <= min(TL_TOPK_MAX, V) most likely
+ *               tokens, larger logit first and the lower index first among
+ *               equal ones; -1 and -inf where fewer tokens have a
+ *               probability.  K = 0: none.
+ * One pass over the logits.  The per-token form of the reference's scoring
+ * commands: cmd_score, tinylm.c:4104-4198; cmd_nll, 4494-4537. */
+int tl_token_logprobs(const void *logits, int dtype, long long ld, const int *ids, int N, int V, float temperature,
+                      float *logp, float *entropy, float *stats, int K, int *top_ids, float *top_logp);
+/* Gradient of sum_n dlogp[n] logp[n] + dentropy[n] entropy[n] in the logits,
+ * written over dlogits (the logits' type, row stride ldd >= V):
+ *   dz_v = (dlogp (1[v = id] - p_v) - dentropy p_v (log p_v + H)) / temperature
+ * with stats and entropy of tl_token_logprobs at the same temperature.  dlogp
+ * (with ids) or dentropy (with entropy) may be NULL.  dlogits may be logits
+ * itself (ldd = ld); other overlap is TL_EINVAL.  A row to which nothing comes
+ * back (dlogp and dentropy 0, or an id of -1) gets zeros and is not read. */
+int tl_token_logprobs_bwd(void *dlogits, long long ldd, const void *logits, int dtype, long long ld, const int *ids,
+                          int N, int V, float temperature, const float *stats, const float *entropy,
+                          const float *dlogp, const float *dentropy);
+/* Distillation from a teacher's K most likely tokens a row: t_ids[n][K]
+ * (-1: padding) and t_vals[n][K], e.g. top_ids and top_logp of
+ * tl_token_logprobs; 1 <= K <= min(TL_TOPK_MAX, V).
+ *   tail 0: q = softmax(t_vals / temperature) over the row's tokens (logits
+ *           or log probabilities, the same result);
+ *   tail 1: t_vals are log probabilities at `temperature`, q = exp(t_vals),
+ *           and the mass they leave, 1 - sum q, is one more class: the tail,
+ *           whose student probability is that of all tokens not named.  A
+ *           tail below 2^-20 (the rounding of fp32 values) is 0.
+ * Entries naming the same token add up.  With p the student's distribution at
+ * `temperature`:
+ *   loss[n] = weight[n] sum q log(q / p)           (weight NULL: 1)
+ *   dlogits = gradient of scale * sum_n loss[n], written over dlogits (the
+ *             logits' type, row stride ldd; may be logits itself with ldd = ld)
+ * Either of loss and dlogits may be NULL.  A row of weight 0 gives 0 and is
+ * not read, a row without teacher tokens gives 0 where there is no tail.  A
+ * token that the teacher names and the student gives probability 0 makes the
+ * loss +inf, a NaN or +inf among the row's t_vals (or logits) its results NaN.
+ * No counterpart in the reference, whose loss knows one target a
+ * token (tinylm.c:1019-1028). */
+int tl_distill_topk(const void *logits, int dtype, long long ld, const int *t_ids, const float *t_vals, int K, int N,
+                    int V, float temperature, int tail, const float *weight, float scale, float *loss, void *dlogits,
+                    long long ldd);
+
 /* ------------------------------------- training loop: host-side pieces */
 /* Checkpoints in the reference's formats.  Buffers may be host or device
  * memory (device data is staged through the host).

@@ -17,8 +17,12 @@ TL_ENOINIT = -6
 TL_EPTR = -7
 TL_ENOMEM = -8
 TL_ZERO1_ALIGN = 4096
+TL_F32, TL_BF16, TL_F16 = 0, 1, 2
+TL_TOPK_MAX = 128
+TL_VOCAB_MAX = 262144
 
 _c_int, _c_size, _c_float, _c_void_p = ctypes.c_int, ctypes.c_size_t, ctypes.c_float, ctypes.c_void_p
+_c_longlong = ctypes.c_longlong
 
 # name -> (restype, argtypes); pointers are passed as integers (void*).
 SIGNATURES = {
@@ -83,6 +87,12 @@ SIGNATURES = {
     "tl_model_step_zero1": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                                      _c_void_p, _c_void_p, _c_int, _c_float, _c_int, _c_float, _c_void_p,
                                      _c_void_p]),
+    "tl_token_logprobs": (_c_int, [_c_void_p, _c_int, _c_longlong, _c_void_p, _c_int, _c_int, _c_float, _c_void_p,
+                                   _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p]),
+    "tl_token_logprobs_bwd": (_c_int, [_c_void_p, _c_longlong, _c_void_p, _c_int, _c_longlong, _c_void_p, _c_int,
+                                       _c_int, _c_float, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "tl_distill_topk": (_c_int, [_c_void_p, _c_int, _c_longlong, _c_void_p, _c_void_p, _c_int, _c_int, _c_int,
+                                 _c_float, _c_int, _c_void_p, _c_float, _c_void_p, _c_void_p, _c_longlong]),
     "tl_zero1_padded": (_c_size, [_c_size, _c_int]),
     "tl_dist_unique_id": (_c_int, [_c_void_p]),
     "tl_dist_init": (_c_int, [_c_int, _c_int, _c_void_p]),

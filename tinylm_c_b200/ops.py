@@ -156,5 +156,122 @@ def clip_adamw(P, G, M, V, n, lr, b1, b2, wd, t, max_norm=1.0, norm_out=None):
                                    n, lr, b1, b2, wd, int(t), max_norm, no))
 
 
+_ROW_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # TL_F32, TL_BF16, TL_F16
+
+
+def _rows(t, name, N, V):
+    """(pointer, row stride) of N rows of V logits: a tensor [>= N, >= V] whose rows are dense, or a
+    contiguous one of at least N*V elements."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a CUDA tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: CPU tensor given; libtinylm_cuda computes on the GPU only")
+    if t.dtype not in _ROW_DTYPES:
+        raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    if t.dim() == 2:
+        if t.shape[0] < N or t.shape[1] < V:
+            raise ValueError(f"{name}: shape {tuple(t.shape)}, call needs [{N}, {V}]")
+        if V > 1 and t.stride(1) != 1:
+            raise ValueError(f"{name}: rows must be dense (stride {t.stride(1)} along them)")
+        ld = t.stride(0) if N > 1 else V
+        if ld < V:
+            raise ValueError(f"{name}: row stride {ld} below V = {V}")
+        return t.data_ptr(), ld
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: must be two-dimensional or contiguous")
+    if t.numel() < N * V:
+        raise ValueError(f"{name}: has {t.numel()} elements, call needs {N * V}")
+    return t.data_ptr(), V
+
+
+def _vec(t, name, numel, dtype=torch.float32):
+    """Pointer of a contiguous CUDA tensor of at least numel elements; None passes through."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a CUDA tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: CPU tensor given; libtinylm_cuda computes on the GPU only")
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: must be contiguous")
+    if t.numel() < numel:
+        raise ValueError(f"{name}: has {t.numel()} elements, call needs {numel}")
+    return t.data_ptr()
+
+
+def _call_on(t, name, *args):
+    """Entry point `name` on t's device and torch's current stream there."""
+    if t.device.index == torch.cuda.current_device():
+        _prep(t)
+        check(getattr(lib(), name)(*args))
+        return
+    with torch.cuda.device(t.device):
+        _prep(t)
+        check(getattr(lib(), name)(*args))
+
+
+def _sizes(N, V, K):
+    if N < 0 or V < 1 or K < 0:
+        raise ValueError(f"bad sizes N = {N}, V = {V}, K = {K}")
+
+
+def token_logprobs(logits, ids, N, V, logp, entropy=None, stats=None, K=0, top_ids=None, top_logp=None,
+                   temperature=1.0):
+    """Scores N rows of V logits (fp32, bf16 or fp16, any row stride).
+
+    logp[n] = log p(ids[n]) (0 where ids[n] is -1; ids and logp may both be
+    None), entropy[n], stats[n][2] (what token_logprobs_bwd needs) and the K
+    most likely tokens top_ids[n][K] / top_logp[n][K].  ids and top_ids are
+    int32, every other output float32; outputs left None are not computed.
+    See tl_token_logprobs in tinylm_cuda.h for masked, empty and NaN rows.
+    """
+    _sizes(N, V, K)
+    z, ld = _rows(logits, "logits", N, V)
+    _call_on(logits, "tl_token_logprobs", z, _ROW_DTYPES[logits.dtype], ld, _vec(ids, "ids", N, torch.int32), N, V,
+             temperature, _vec(logp, "logp", N), _vec(entropy, "entropy", N), _vec(stats, "stats", 2 * N), K,
+             _vec(top_ids, "top_ids", N * K, torch.int32), _vec(top_logp, "top_logp", N * K))
+
+
+def token_logprobs_bwd(dlogits, logits, ids, N, V, stats, dlogp, entropy=None, dentropy=None, temperature=1.0):
+    """dlogits = gradient of sum dlogp*logp + dentropy*entropy in the logits.
+
+    stats and entropy are those of token_logprobs at the same temperature;
+    dlogp (with ids) or dentropy (with entropy) may be None.  dlogits has the
+    logits' type and may be the logits tensor itself.
+    """
+    _sizes(N, V, 0)
+    z, ld = _rows(logits, "logits", N, V)
+    dz, ldd = _rows(dlogits, "dlogits", N, V)
+    if dlogits.dtype != logits.dtype:
+        raise TypeError(f"dlogits: expected {logits.dtype}, got {dlogits.dtype}")
+    _call_on(logits, "tl_token_logprobs_bwd", dz, ldd, z, _ROW_DTYPES[logits.dtype], ld,
+             _vec(ids, "ids", N, torch.int32), N, V, temperature, _vec(stats, "stats", 2 * N),
+             _vec(entropy, "entropy", N), _vec(dlogp, "dlogp", N), _vec(dentropy, "dentropy", N))
+
+
+def distill_topk(logits, t_ids, t_vals, N, V, K, loss, dlogits=None, weight=None, scale=1.0, temperature=1.0,
+                 tail=False):
+    """KL divergence of N student rows from a teacher's K most likely tokens.
+
+    loss[n] = weight[n] * sum q log(q / p); dlogits, if given, receives the
+    gradient of scale * sum(loss) and may be the logits tensor itself.  q is
+    the softmax of t_vals / temperature over the row's tokens, or, with
+    tail=True, exp(t_vals) (log probabilities at this temperature) and the
+    mass they leave as one more class.  t_ids is int32 [N][K] with -1 as
+    padding, t_vals float32 [N][K]; either of loss and dlogits may be None.
+    See tl_distill_topk in tinylm_cuda.h.
+    """
+    _sizes(N, V, K)
+    z, ld = _rows(logits, "logits", N, V)
+    dz, ldd = (None, 0) if dlogits is None else _rows(dlogits, "dlogits", N, V)
+    if dlogits is not None and dlogits.dtype != logits.dtype:
+        raise TypeError(f"dlogits: expected {logits.dtype}, got {dlogits.dtype}")
+    _call_on(logits, "tl_distill_topk", z, _ROW_DTYPES[logits.dtype], ld,
+             _vec(t_ids, "t_ids", N * K, torch.int32), _vec(t_vals, "t_vals", N * K), K, N, V, temperature, int(tail),
+             _vec(weight, "weight", N), scale, _vec(loss, "loss", N), dz, ldd)
+
+
 def sync():
     check(lib().tl_sync())
