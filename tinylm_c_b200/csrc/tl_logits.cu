@@ -19,31 +19,57 @@ RowPlan plan_rows(const DeviceCtx *c, const LogitRows &z, int K) {
   const bool one = (z.ld * es) % 16 == 0 || z.N == 1;
   const int mis = one ? (int)(reinterpret_cast<uintptr_t>(z.p) & 15) / es : ev - 1;
   const int nch = (z.V + mis + ev - 1) / ev;
-  RowPlan p{512, 1};
-  if (nch <= 32 * lg::NV && K <= 16) p.threads = 32;
-  else if (nch <= 128 * lg::NV) p.threads = 128;
-  else if (nch <= 256 * lg::NV) p.threads = 256;
-  else p.blocks = (nch + 512 * lg::NV - 1) / (512 * lg::NV);
+  int blocks = (nch + 2047) / 2048;
+  if (blocks > lg::MAX_CLUSTER) blocks = lg::MAX_CLUSTER;
   // few rows: more blocks a row
-  while ((long long)z.N * p.blocks * 2 <= c->num_sms && p.blocks * 2 <= 8 && nch / p.blocks >= 512) p.blocks *= 2;
-  if (p.blocks > 1) p.threads = (nch + p.blocks - 1) / p.blocks <= 512 ? 256 : 512;
+  while ((long long)z.N * blocks * 2 <= c->num_sms && blocks * 2 <= 8 && nch / blocks >= 512) blocks *= 2;
+  const int per = (nch + blocks - 1) / blocks;
+  RowPlan p{256, blocks, {z.p, z.ld, z.N, z.V, per, 2, (per + 7) / 8 * 8, 0}};
+  if (per > 2048 + 256) p.threads = 512;
+  else if (blocks == 1 && per <= 256 && K <= 16) p.threads = 32;
+  else if (per <= 1024) p.threads = 128;
+  if (p.threads == 32) p.l.stages = 4;
+  p.l.ragged = !one || mis || (z.V % ev) != 0;
   return p;
 }
 
-int launch_rows_cluster(const void *kernel, DeviceCtx *c, int N, int threads, int blocks, void *args) {
-  if (blocks > lg::MAX_CLUSTER || (long long)N * blocks > 0x7FFFFFFFLL)
-    return set_error(TL_EINVAL, "N = %d rows of %d blocks are too many for one launch", N, blocks);
-  if (blocks > 8) TL_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+int launch_rows(const void *kernel, DeviceCtx *c, const RowPlan &p, int more_smem, Resident *seen, void *args) {
+  constexpr int kMaxDynamic = 220 * 1024;          // of 227 KB a block may have, less the kernels' static part
+  const int smem = p.l.stages * p.l.chunks * 16 + more_smem;
+  if (smem > kMaxDynamic) return set_error(TL_EINVAL, "rows need %d bytes of shared memory a block", smem);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(N * blocks));
-  cfg.blockDim = dim3((unsigned)threads);
+  cfg.blockDim = dim3((unsigned)p.threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = c->stream;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = (unsigned)blocks;
+  at.val.clusterDim.x = (unsigned)p.blocks;
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
+  if (p.blocks > 1) {
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+  }
+  if (!seen->ready) {
+    TL_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynamic));
+    TL_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    seen->ready = 1;
+  }
+  int fit = 0;
+  for (const Resident::Shape &s : seen->of)
+    if (s.threads == p.threads && s.blocks == p.blocks && s.smem == smem) fit = s.fit;
+  if (!fit) {
+    if (p.blocks == 1) {
+      TL_TRY_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, p.threads, (size_t)smem));
+      fit *= c->num_sms;
+    } else {
+      cfg.gridDim = dim3((unsigned)p.blocks);
+      TL_TRY_CUDA(cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg));
+    }
+    if (fit < 1) return set_error(TL_ECUDA, "%d blocks of %d threads and %d bytes do not fit", p.blocks, p.threads, smem);
+    seen->of[seen->next] = Resident::Shape{p.threads, p.blocks, smem, fit};
+    seen->next = (seen->next + 1) % Resident::N;
+  }
+  cfg.gridDim = dim3((unsigned)((p.l.N < fit ? p.l.N : fit) * p.blocks));
   void *argv[1] = {args};
   TL_TRY_CUDA(cudaLaunchKernelExC(&cfg, kernel, argv));
   return TL_OK;

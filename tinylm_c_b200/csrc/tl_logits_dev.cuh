@@ -1,19 +1,24 @@
 // tl_logits_dev.cuh -- device pieces shared by the vocabulary-row kernels: a
-// row's slice held in registers, the softmax statistics, the exchange between
+// row's share in shared memory, the softmax statistics, the exchange between
 // the blocks of a row.
 //
-// A row is held as 16-byte chunks of memory, counted from the aligned address
-// at or below its start, so a row of any element alignment is loaded and
-// stored 16 bytes at a time; only the (at most two) chunks that reach past
-// the row's ends go element by element.  A row is owned by one block, or by
-// the blocks of one cluster, each with a contiguous range of chunks; thread t
-// of TH holds chunks t, t + TH, ... of its block's range, NV of them.
+// A row is handled as 16-byte chunks of memory, counted from the aligned
+// address at or below its start, so a row of any element alignment is moved 16
+// bytes at a time; elements of a neighbouring row in its first and last chunk
+// are set to -inf once they are in shared memory, and only chunks that reach
+// past the whole tensor go element by element.  A row is owned by one block,
+// or by the blocks of one cluster, each with a contiguous share of its chunks.
+// The blocks stay on the GPU and take rows in turn; while one row is worked on
+// the share of the next is on its way by a bulk copy into another stage of
+// shared memory, so the memory system is busy throughout.  A row is read from
+// memory once, however often a kernel goes over it.
 #pragma once
 #include <cfloat>
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "tl_logits.cuh"
+#include "tl_tc_ptx.cuh"
 
 namespace tl {
 namespace lg {
@@ -24,8 +29,9 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr unsigned FULL = 0xFFFFFFFFu;
 constexpr int MAX_CLUSTER = 16;
-// Chunks held by one thread.
-constexpr int NV = 8;
+constexpr int MAX_THREADS = 512, MAX_WARPS = MAX_THREADS / 32, MAX_STAGES = 4;
+constexpr int ERR_COPY = 90;                       // error word: a bulk copy did not arrive in time
+constexpr int ERR_TOKEN = 100;                     // a token id outside [0, V)
 
 // ------------------------------------------------------------- arithmetic
 // Two fp32 operations in one instruction (sm_100's packed pairs), each
@@ -67,10 +73,11 @@ __device__ __forceinline__ float bounded(float x) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(-1e30f));
   return r;
 }
+// The warp's largest value (NaN only if all are).
 __device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, o));
-  return v;
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
 }
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -83,6 +90,7 @@ template <typename T> struct Elem;
 template <> struct Elem<float> {
   static constexpr int EV = 4;                       // elements of a chunk
   static constexpr unsigned FILL = 0xFF800000u;      // -inf in every element
+  static __device__ __forceinline__ float none() { return __uint_as_float(FILL); }
   static __device__ __forceinline__ float to_f(float x) { return x; }
   static __device__ __forceinline__ float from_f(float x) { return x; }
   static __device__ __forceinline__ void unpack(const uint4 &c, float (&f)[EV]) {
@@ -103,6 +111,7 @@ template <> struct Elem<float> {
 template <> struct Elem<__nv_bfloat16> {
   static constexpr int EV = 8;
   static constexpr unsigned FILL = 0xFF80FF80u;
+  static __device__ __forceinline__ __nv_bfloat16 none() { return __ushort_as_bfloat16(0xFF80); }
   static __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
   static __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
   static __device__ __forceinline__ void unpack(const uint4 &c, float (&f)[EV]) {
@@ -132,6 +141,7 @@ template <> struct Elem<__nv_bfloat16> {
 template <> struct Elem<__half> {
   static constexpr int EV = 8;
   static constexpr unsigned FILL = 0xFC00FC00u;
+  static __device__ __forceinline__ __half none() { return __ushort_as_half(0xFC00); }
   static __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
   static __device__ __forceinline__ __half from_f(float x) { return __float2half_rn(x); }
   static __device__ __forceinline__ void unpack(const uint4 &c, float (&f)[EV]) {
@@ -198,48 +208,131 @@ template <typename T> struct Chunks {
   }
 };
 
-// This thread's chunks of [c0, c1): all loads in flight together.
-template <typename T, int TH>
-__device__ __forceinline__ void load_slice(const Chunks<T> &r, int c0, int c1, uint4 (&x)[NV]) {
-  const int lo = max(c0, r.full0), hi = min(c1, r.full1), t = threadIdx.x;
-#pragma unroll
-  for (int i = 0; i < NV; i++) {
-    const int c = c0 + i * TH + t;
-    x[i] = make_uint4(Elem<T>::FILL, Elem<T>::FILL, Elem<T>::FILL, Elem<T>::FILL);
-    if (c >= lo && c < hi) x[i] = __ldcg(r.base + c);
+// The tensor's rows and how they are shared out, as the host lays it out: each
+// of a row's blocks has `per` chunks (the last one what is left) and `stages`
+// buffers of `chunks` >= per chunks; `ragged`: some row's ends do not fill
+// their chunks.
+struct Layout {
+  const void *z;
+  long long ld;
+  int N, V, per, stages, chunks, ragged;
+};
+template <typename T> struct Rows {
+  const T *z;
+  long long ld;
+  int V, c0, per;
+  uintptr_t end;                       // one past the last row
+  bool ragged;
+  __device__ __forceinline__ Rows(const Layout &l, int rank)
+      : z(static_cast<const T *>(l.z)), ld(l.ld), V(l.V), c0(rank * l.per), per(l.per),
+        end(reinterpret_cast<uintptr_t>(z + ((long long)(l.N - 1) * ld + V))), ragged(l.ragged) {}
+};
+// A block's share of a row: chunks [c0, c0 + cnt), in shared memory from 0.
+template <typename T> struct Share {
+  Chunks<T> r;
+  int c0, cnt;
+  __device__ __forceinline__ Share(const Rows<T> &t, int n) : r(t.z + (size_t)n * t.ld, t.V) {
+    c0 = t.c0;
+    cnt = max(0, min(r.n - c0, t.per));
   }
-  // the row's first and last chunk, where they reach past it
+  // Whether a chunk lies inside the tensor as a whole, so that it may be copied.
+  static __device__ __forceinline__ bool inside(const Rows<T> &t, const uint4 *p) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+    return a >= reinterpret_cast<uintptr_t>(t.z) && a + 16 <= t.end;
+  }
+};
+
+// Rows on their way into `stages` buffers of `bytes` each (a multiple of 128).
+// One thread issues the copies; all wait for them.
+template <typename T> struct Pipe {
+  uint4 *buf;                          // stage 0
+  int stages, stage_chunks;
+  uint64_t *full;                      // a barrier a stage
+  int *abort_flag;                     // a copy did not arrive: nothing is waited for or copied any more
+  int *err;
+  int at = 0, phase = 0;               // the stage of the row at hand, its barrier's parity
+  __device__ __forceinline__ void init() {
+    for (int i = 0; i < stages; i++) tc::mbar_init(tc::smem_u32(&full[i]), 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __device__ __forceinline__ uint4 *stage() const { return buf + (size_t)at * stage_chunks; }
+  __device__ __forceinline__ void next() {
+    if (++at == stages) { at = 0; phase ^= 1; }
+  }
+  // Row n's share into stage s (`read` false: nothing is copied, the stage is
+  // full at once).  The stage's earlier readers have passed a barrier.  The
+  // tensor's first and last chunk, where it does not fill them, are written
+  // by the calling thread.
+  __device__ __forceinline__ void issue(const Rows<T> &t, int n, int s, bool read) const {
+    const uint32_t bar = tc::smem_u32(&full[s]);
+    if (*(volatile int *)abort_flag) return;
+    int lo = 0, hi = 0, c0 = 0;
+    const uint4 *base = nullptr;
+    if (read) {
+      const Share<T> sh(t, n);
+      base = sh.r.base;
+      c0 = lo = sh.c0;
+      hi = sh.c0 + sh.cnt;
+      uint4 *st = buf + (size_t)s * stage_chunks;
+      if (lo < hi && !Share<T>::inside(t, base + lo)) {
+        st[0] = sh.r.load_edge(lo);
+        lo++;
+      }
+      if (lo < hi && !Share<T>::inside(t, base + hi - 1)) {
+        hi--;
+        st[hi - c0] = sh.r.load_edge(hi);
+      }
+    }
+    const uint32_t bytes = (uint32_t)(hi - lo) * 16u;
+    // what other threads read of the stage comes before what the copy writes
+    tc::fence_proxy_async();
+    tc::mbar_arrive_expect_tx(bar, bytes);
+    if (bytes)
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                       tc::smem_u32(buf + (size_t)s * stage_chunks + (lo - c0))),
+                   "l"(__cvta_generic_to_global(base + lo)), "r"(bytes), "r"(bar)
+                   : "memory");
+  }
+  // The row at hand is in shared memory, its ends masked; the thread that
+  // reads an end chunk (t of n threads reads chunks t, t + n, ...) masks it.
+  // After an expired wait the kernel runs on over what there is, its copies
+  // and waits over, and the error word says so: leaving would strand the
+  // other blocks of the row.
+  __device__ __forceinline__ void wait(const Rows<T> &t, const Share<T> &sh) const {
+    tc::mbar_wait(tc::smem_u32(&full[at]), phase, abort_flag, err, ERR_COPY);
+    if (!t.ragged) return;
+    uint4 *st = stage();
 #pragma unroll
-  for (int k = 0; k < 2; k++) {
-    const int c = k ? r.n - 1 : 0;
-    const bool reaches = k ? r.full1 < r.n && (r.n > 1 || r.full0 == 0) : r.full0 == 1;
-    if (reaches && c >= c0 && c < c1 && (c - c0) % TH == t) {
-      const uint4 v = r.load_edge(c);
-      const int at = (c - c0) / TH;
-#pragma unroll
-      for (int i = 0; i < NV; i++)
-        if (i == at) x[i] = v;
+    for (int k = 0; k < 2; k++) {
+      const int c = k ? sh.r.n - 1 : 0;
+      const bool partial = k ? sh.r.full1 < sh.r.n && (sh.r.n > 1 || sh.r.full0 == 0) : sh.r.full0 == 1;
+      if (partial && c >= sh.c0 && c < sh.c0 + sh.cnt && (c - sh.c0) % (int)blockDim.x == (int)threadIdx.x) {
+        T *e = reinterpret_cast<T *>(st + (c - sh.c0));
+        const int v = sh.r.first(c);
+        for (int i = 0; i < Elem<T>::EV; i++)
+          if (v + i < 0 || v + i >= sh.r.V) e[i] = Elem<T>::none();
+        tc::fence_proxy_async();       // a later copy into this stage comes after these writes
+      }
     }
   }
-}
+};
 
 // ------------------------------------------------- statistics and exchange
 // Of a part of a row: m its largest logit (at least -FLT_MAX), s the sum of
-// e = 2^((z - m) c) and t that of e (z - m) c, c = log2(e) / temperature; w is
-// free for the caller.
+// e = 2^((z - m) c) and t that of e (z - m) c, c = log2(e) / temperature; w a
+// value of which the part's elements hold at least some known number of larger
+// ones (-inf: none known).
 struct Part {
   float m, s, t, w;
 };
-__device__ __forceinline__ Part no_part(float w) { return Part{-FLT_MAX, 0.0f, 0.0f, w}; }
+__device__ __forceinline__ Part no_part() { return Part{-FLT_MAX, 0.0f, 0.0f, -INFINITY}; }
 // The parts of lanes 0..15 as one; every lane of both halves gets the same
 // bits (each step adds the same two values on both sides).
 template <bool ENT> __device__ __forceinline__ Part join_lanes(Part p, float c) {
   float m = p.m;
 #pragma unroll
-  for (int o = 8; o; o >>= 1) {
-    m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
-    p.w = fminf(p.w, __shfl_xor_sync(FULL, p.w, o));
-  }
+  for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
   const float d = bounded((p.m - m) * c), f = exp2_fast(d);
   if (ENT) p.t = f * (p.t + p.s * d);
   p.s *= f;
@@ -252,29 +345,48 @@ template <bool ENT> __device__ __forceinline__ Part join_lanes(Part p, float c) 
   return p;
 }
 
-// A warp's part of the row from its lanes' chunks; `lane_max` is this lane's
-// largest logit (-inf if it has none).  cnt: chunks of the block's range.
-template <typename T, int TH, bool ENT>
-__device__ __forceinline__ Part warp_part(const uint4 (&x)[NV], int cnt, float lane_max, float c) {
+// The j-th largest of the values of N neighbouring lanes, 1 <= j <= N: a
+// bitonic sort in descending order.
+template <int N> __device__ __forceinline__ float nth_largest(float v, int j) {
+  const int lane = threadIdx.x & (N - 1);
+#pragma unroll
+  for (int k = 2; k <= N; k <<= 1)
+#pragma unroll
+    for (int o = k >> 1; o; o >>= 1) {
+      const float u = __shfl_xor_sync(FULL, v, o);
+      v = ((lane & o) == 0) == ((lane & k) == 0) ? fmaxf(v, u) : fminf(v, u);
+    }
+  return __shfl_sync(FULL, v, j - 1);
+}
+
+// This thread's largest logit of the share (-inf if it has none).
+template <typename T> __device__ __forceinline__ float thread_max(const uint4 *st, int cnt) {
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < cnt; i += blockDim.x) m = fmaxf(m, Elem<T>::max_of(st[i]));
+  return m;
+}
+// A warp's part of the row; `top` is this thread's largest logit.
+template <typename T, bool ENT>
+__device__ __forceinline__ Part warp_part(const uint4 *st, int cnt, float top, float c) {
   constexpr int EV = Elem<T>::EV;
-  const float m = fmaxf(warp_max(lane_max), -FLT_MAX);
+  const float m = fmaxf(warp_max(top), -FLT_MAX);
   const f32x2 nm = pack2(-m, -m), cc = pack2(c, c);
   f32x2 s2 = pack2(0.0f, 0.0f), t2 = s2;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < cnt; i += blockDim.x) {
+    float f[EV];
+    Elem<T>::unpack(st[i], f);
 #pragma unroll
-  for (int i = 0; i < NV; i++)
-    if (i * TH < cnt) {
-      float f[EV];
-      Elem<T>::unpack(x[i], f);
-#pragma unroll
-      for (int e = 0; e < EV; e += 2) {
-        f32x2 d = mul2(add2(pack2(f[e], f[e + 1]), nm), cc);
-        float d0, d1;
-        unpack2(d, d0, d1);
-        const f32x2 ex = pack2(exp2_fast(d0), exp2_fast(d1));
-        s2 = add2(s2, ex);
-        if (ENT) t2 = fma2(ex, pack2(bounded(d0), bounded(d1)), t2);
-      }
+    for (int e = 0; e < EV; e += 2) {
+      const f32x2 d = mul2(add2(pack2(f[e], f[e + 1]), nm), cc);
+      float d0, d1;
+      unpack2(d, d0, d1);
+      const f32x2 ex = pack2(exp2_fast(d0), exp2_fast(d1));
+      s2 = add2(s2, ex);
+      if (ENT) t2 = fma2(ex, pack2(bounded(d0), bounded(d1)), t2);
     }
+  }
   float a, b;
   unpack2(s2, a, b);
   Part p;
@@ -282,16 +394,8 @@ __device__ __forceinline__ Part warp_part(const uint4 (&x)[NV], int cnt, float l
   p.s = warp_sum(a + b);
   unpack2(t2, a, b);
   p.t = ENT ? warp_sum(a + b) : 0.0f;
-  p.w = 0.0f;
+  p.w = -INFINITY;
   return p;
-}
-template <typename T, int TH>
-__device__ __forceinline__ float lane_max_of(const uint4 (&x)[NV], int cnt) {
-  float m = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < NV; i++)
-    if (i * TH < cnt) m = fmaxf(m, Elem<T>::max_of(x[i]));
-  return m;
 }
 
 // The blocks of a row.  One block: barriers are the block's and no memory is
@@ -316,36 +420,54 @@ template <> struct Team<true> {
   }
 };
 
-// Every warp's part (in part[], written by its lane 0) joined over the row's
-// blocks; every thread gets the same result.  `none` is w where there is no
-// part.  The cluster's blocks have arrived at its first barrier before
-// (Team::arrive), which is waited for here: memory of a block that has not
-// started is not written.
-template <bool CL, int W, bool ENT>
-__device__ __forceinline__ Part join_row(const Part *part, Part *from, float none, float c) {
-  using TM = Team<CL>;
+// The parts of a row's warps (one block) or blocks (cluster) as one; for every
+// lane of the calling warp.
+template <bool ENT> __device__ __forceinline__ Part join_all(const Part *part, int count, float c) {
   const int lane = threadIdx.x & 15;
+  Part p = no_part();
+  if (lane < count) p = part[lane];
+  return join_lanes<ENT>(p, c);
+}
+// Hands the block's part to the row's blocks (from[], by rank) and waits for
+// theirs; the block's warps have written part[] before.  w becomes the g-th
+// largest of the warps', +inf where g is 0.  The caller takes part[] and
+// from[] in turn from two buffers: a barrier lies between a row's reads of one
+// and the next write of it.
+template <bool ENT>
+__device__ __forceinline__ void meet(const Part *part, Part *from, int g, float c) {
+  using TM = Team<true>;
   __syncthreads();
-  if (!CL) return W == 1 ? part[0] : join_lanes<ENT>(lane < W ? part[lane] : no_part(none), c);
-  TM::wait();
   if (threadIdx.x < 32) {
-    const Part p = join_lanes<ENT>(lane < W ? part[lane] : no_part(none), c);
+    Part p = join_all<ENT>(part, blockDim.x >> 5, c);
+    p.w = INFINITY;
+    if (g) p.w = nth_largest<16>((threadIdx.x & 15) < (blockDim.x >> 5) ? part[threadIdx.x & 15].w : -INFINITY, g);
     if (threadIdx.x < TM::size()) *TM::at(&from[TM::rank()], threadIdx.x) = p;
   }
   TM::sync();
-  return join_lanes<ENT>(lane < (int)TM::size() ? from[lane] : no_part(none), c);
 }
 
 }  // namespace lg
 
 // ------------------------------------------------------------ launch plan
-// How a row is laid over the GPU: `threads` a block, `blocks` a row (more than
+// How rows are laid over the GPU: `threads` a block, `blocks` a row (more than
 // one: a cluster).
 struct RowPlan {
   int threads, blocks;
+  lg::Layout l;
 };
 RowPlan plan_rows(const DeviceCtx *c, const LogitRows &z, int K);
-// Launches N clusters of `blocks` blocks; `args` is the kernel's one argument.
-int launch_rows_cluster(const void *kernel, DeviceCtx *c, int N, int threads, int blocks, void *args);
+// Launches a kernel over N rows: as many blocks (clusters of `blocks`) as the
+// GPU holds at once, each taking rows in turn.  `more_smem` bytes of dynamic
+// shared memory follow the stages, `args` is the kernel's one argument, `seen`
+// belongs to the kernel and the device: how many fit, for its latest shapes.
+struct Resident {
+  static constexpr int N = 16;
+  struct Shape {
+    int threads, blocks, smem, fit;
+  };
+  int ready, next;
+  Shape of[N];
+};
+int launch_rows(const void *kernel, DeviceCtx *c, const RowPlan &p, int more_smem, Resident *seen, void *args);
 
 }  // namespace tl

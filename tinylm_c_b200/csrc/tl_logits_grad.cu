@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(256) token_logprobs_bwd_kernel(const GradArgs 
   const int c0 = seg * (TPR * CPT) + t;
   int id = a.dlogp ? a.ids[n] : -1;
   if (id != -1 && (unsigned)id >= (unsigned)a.V) {
-    if (c0 == 0) atomicExch(a.err, 100);
+    if (c0 == 0) atomicExch(a.err, ERR_TOKEN);
     id = -1;
   }
   const float m = a.stats[2 * n], ls = a.stats[2 * n + 1];
@@ -97,11 +97,10 @@ __global__ void __launch_bounds__(256) token_logprobs_bwd_kernel(const GradArgs 
 
 // ------------------------------------------------------------ distillation
 struct DistillArgs {
-  const void *z;
-  long long ld;
+  Layout l;
   const int *t_ids;
   const float *t_vals;
-  int K, V;
+  int K;
   float c, inv_t;
   const float *weight;
   float scale;
@@ -116,218 +115,224 @@ struct DistillArgs {
 // + q_r (log q_r - log p_r), p_r = sum of p over the others; Q = sum q + q_r.
 //   named v:  dL/dy_v = Q p_v - q_v
 //   others:   dL/dy_v = p_v (Q - q_r / p_r)
-// The row is loaded once and stays in registers; with a tail the named tokens
-// are taken out of it first (a bit for each element of the block's slice), so
-// that p_r is summed and never 1 - sum p, which loses all its digits for a
-// confident student.  All others' gradients are then one factor times e_v;
-// the named tokens' are written over them at the end.
-template <typename T, int TH, bool CL, bool TAIL>
-__global__ void __launch_bounds__(TH, 1024 / TH) distill_kernel(const DistillArgs a) {
+// The row is read once.  With a tail the named tokens are taken out of it (set
+// to -inf in shared memory) before its statistics, so that p_r is summed and
+// never 1 - sum p, which loses all its digits for a confident student.  All
+// others' gradients are then one factor times e_v; the named tokens' are
+// written over them at the end.
+template <typename T, bool CL, bool TAIL>
+__global__ void __launch_bounds__(MAX_THREADS, 2) distill_kernel(const DistillArgs a) {
   using TM = Team<CL>;
-  constexpr int W = TH / 32, EV = Elem<T>::EV, KL = TL_TOPK_MAX / 32;
-  __shared__ Part s_part[W], s_from[MAX_CLUSTER];
-  __shared__ int s_id[TL_TOPK_MAX];              // -1: padding
-  __shared__ float s_q[TL_TOPK_MAX], s_z[TL_TOPK_MAX];
-  __shared__ float s_qv[TL_TOPK_MAX];            // mass of the token an entry stands for, -1 if it stands for none
-  __shared__ float s_sum[2];                     // sum of q, the tail
-  __shared__ __align__(8) unsigned char s_named[TAIL ? TH * NV : 8];   // a bit an element, a byte a chunk
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const unsigned rank = TM::rank(), S = TM::size();
-  const size_t n = CL ? blockIdx.x / S : blockIdx.x;
-  const Chunks<T> r(static_cast<const T *>(a.z) + n * a.ld, a.V);
-  const int per = CL ? (r.n + (int)S - 1) / (int)S : r.n;
-  const int c0 = (int)rank * per, c1 = min(r.n, c0 + per), cnt = c1 - c0;
-  const Chunks<T> o(static_cast<const T *>(a.dz) + (a.dz ? n * a.ldd : 0), a.V);
-  const float w = a.weight ? a.weight[n] : 1.0f;
-  const bool same = o.mis == r.mis;
-  auto store = [&](int c, const float (&f)[EV]) {
-    if (same && c >= r.full0 && c < r.full1) {
-      o.base[c] = Elem<T>::pack(f);
-    } else {
-      const int v = r.first(c);
-#pragma unroll
-      for (int e = 0; e < EV; e++)
-        if (v + e >= 0 && v + e < a.V) o.row[v + e] = Elem<T>::from_f(f[e]);
-    }
-  };
-  if (w == 0.0f) {                               // a row that does not count is not read
-    if (a.dz) {
-      const float f[EV] = {};
-      for (int c = c0 + tid; c < c1; c += TH) store(c, f);
-    }
-    if (rank == 0 && tid == 0) {
-      if (a.loss) a.loss[n] = 0.0f;
-      if (a.loss64) a.loss64[n] = 0.0;
-    }
-    return;
+  constexpr int EV = Elem<T>::EV, KL = TL_TOPK_MAX / 32;
+  extern __shared__ __align__(128) unsigned char s_dyn[];
+  // two of each, for rows in turn: a barrier of the next row lies between a
+  // row's last reads and the row after that's writes
+  __shared__ Part s_part[2][MAX_WARPS], s_from[2][MAX_CLUSTER];
+  __shared__ float s_sum[2][2];                  // sum of q, the tail
+  __shared__ uint64_t s_full[MAX_STAGES];
+  __shared__ int s_abort;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, TH = blockDim.x;
+  const int S = (int)TM::size();
+  const int rank = (int)TM::rank();
+  const Rows<T> t(a.l, rank);
+  const int N = a.l.N, V = a.l.V, stride = (int)gridDim.x / S, first_row = (int)blockIdx.x / S;
+  Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), a.l.stages, a.l.chunks, s_full, &s_abort, a.err};
+  // the row's entries: token (-1: padding), its q and logit, and the mass of
+  // the token an entry stands for (-1 if it stands for none)
+  float *s_entry = reinterpret_cast<float *>(s_dyn + (size_t)a.l.stages * a.l.chunks * 16);
+  auto counts = [&](int n) { return !a.weight || a.weight[n] != 0.0f; };
+  if (tid == 0) {
+    pipe.init();
+    for (int i = 0; i < a.l.stages; i++)
+      if (first_row + i * stride < N) pipe.issue(t, first_row + i * stride, i, counts(first_row + i * stride));
   }
-  TM::arrive();
-  uint4 x[NV];
-  load_slice<T, TH>(r, c0, c1, x);
-  if (TAIL) {
-    *reinterpret_cast<uint2 *>(&s_named[tid * NV]) = make_uint2(0, 0);
-    __syncthreads();
-  }
-  // ---- the teacher's entries, by the first warp of every block
-  if (warp == 0) {
-    int id[KL];
-    float t[KL], tm = -FLT_MAX;
-#pragma unroll
-    for (int k = 0; k < KL; k++) {
-      const int j = k * 32 + lane;
-      id[k] = -1;
-      t[k] = -INFINITY;
-      if (j < a.K) {
-        id[k] = a.t_ids[n * a.K + j];
-        t[k] = a.t_vals[n * a.K + j];
-      }
-    }
-    float z[KL];
-#pragma unroll
-    for (int k = 0; k < KL; k++) {
-      const int j = k * 32 + lane;
-      if ((unsigned)id[k] >= (unsigned)a.V) {
-        if (id[k] != -1) atomicExch(a.err, 100);
-        id[k] = -1;
-        t[k] = -INFINITY;
-      }
-      z[k] = -INFINITY;
-      if (id[k] >= 0) {
-        z[k] = Elem<T>::to_f(r.row[id[k]]);
-        if (TAIL) {
-          const int at = (id[k] + r.mis) / EV - c0, e = (id[k] + r.mis) % EV;
-          if (at >= 0 && at < cnt)
-            atomicOr(reinterpret_cast<unsigned *>(s_named) + (at >> 2), 1u << ((at & 3) * 8 + e));
-        }
-      }
-      if (j < a.K) s_id[j] = id[k];
-      tm = fmaxf(tm, t[k]);
-    }
-    if (!TAIL) tm = warp_max(tm);
-    float q[KL], sum = 0.0f;
-#pragma unroll
-    for (int k = 0; k < KL; k++) {
-      q[k] = id[k] < 0 ? 0.0f : expf(TAIL ? t[k] : (t[k] - tm) * a.inv_t);
-      sum += q[k];
-    }
-    sum = warp_sum(sum);
-    const float inv = TAIL ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-    for (int k = 0; k < KL; k++) {
-      const int j = k * 32 + lane;
-      if (j < a.K) {
-        s_q[j] = q[k] * inv;
-        s_z[j] = z[k];
-      }
-    }
-    if (lane == 0) {
-      float Q = TAIL || sum == 0.0f ? sum : 1.0f;
-      if (!(sum < INFINITY)) Q = NAN;            // a NaN or +inf among the values
-      const float qr = TAIL ? 1.0f - Q : 0.0f;
-      s_sum[0] = Q;
-      s_sum[1] = qr < TAIL_MIN ? 0.0f : qr;      // NaN stays
-    }
-  }
-  if (TAIL) {
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const unsigned named = s_named[i * TH + tid];
-      if (named) {
-        unsigned u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+  TM::sync();
+  for (int n = first_row, flip = 0; n < N; n += stride, flip ^= 1) {
+    const Share<T> sh(t, n);
+    const Chunks<T> &r = sh.r;
+    const Chunks<T> o(static_cast<const T *>(a.dz) + (a.dz ? (size_t)n * a.ldd : 0), V);
+    const float w = a.weight ? a.weight[n] : 1.0f;
+    const int cnt = sh.cnt, ahead = n + a.l.stages * stride;
+    const bool next_counts = tid == 0 && ahead < N && counts(ahead);
+    uint4 *st = pipe.stage();
+    int *s_id = reinterpret_cast<int *>(s_entry) + flip * 4 * a.K;
+    float *s_q = s_entry + flip * 4 * a.K + a.K, *s_z = s_q + a.K, *s_qv = s_z + a.K;
+    auto store = [&](int c, const float (&f)[EV]) {
+      if (o.mis == r.mis && c >= r.full0 && c < r.full1) {
+        o.base[c] = Elem<T>::pack(f);
+      } else {
+        const int v = r.first(c);
 #pragma unroll
         for (int e = 0; e < EV; e++)
-          if (named >> e & 1) {
-            if (EV == 4) u[e & 3] = Elem<T>::FILL;
-            else u[(e >> 1) & 3] = e & 1 ? (u[(e >> 1) & 3] & 0x0000FFFFu) | (Elem<T>::FILL & 0xFFFF0000u)
-                                         : (u[(e >> 1) & 3] & 0xFFFF0000u) | (Elem<T>::FILL & 0x0000FFFFu);
+          if (v + e >= 0 && v + e < V) o.row[v + e] = Elem<T>::from_f(f[e]);
+      }
+    };
+    if (w == 0.0f) {                             // a row that does not count is not read
+      if (a.dz) {
+        const float f[EV] = {};
+        for (int i = tid; i < cnt; i += TH) store(sh.c0 + i, f);
+      }
+      if (rank == 0 && tid == 0) {
+        if (a.loss) a.loss[n] = 0.0f;
+        if (a.loss64) a.loss64[n] = 0.0;
+      }
+      tc::mbar_wait(tc::smem_u32(&s_full[pipe.at]), pipe.phase, &s_abort, a.err, ERR_COPY);
+      TM::sync();
+      if (tid == 0 && ahead < N) pipe.issue(t, ahead, pipe.at, next_counts);
+      pipe.next();
+      continue;
+    }
+    // ---- the teacher's entries, by the first warp of every block
+    if (warp == 0) {
+      int id[KL];
+      float tv[KL], tm = -FLT_MAX;
+#pragma unroll
+      for (int k = 0; k < KL; k++) {
+        const int j = k * 32 + lane;
+        id[k] = -1;
+        tv[k] = -INFINITY;
+        if (j < a.K) {
+          id[k] = a.t_ids[(size_t)n * a.K + j];
+          tv[k] = a.t_vals[(size_t)n * a.K + j];
+        }
+      }
+      float zk[KL];
+#pragma unroll
+      for (int k = 0; k < KL; k++) {
+        if ((unsigned)id[k] >= (unsigned)V) {
+          if (id[k] != -1) atomicExch(a.err, ERR_TOKEN);
+          id[k] = -1;
+          tv[k] = -INFINITY;
+        }
+        zk[k] = id[k] >= 0 ? Elem<T>::to_f(r.row[id[k]]) : -INFINITY;
+        tm = fmaxf(tm, tv[k]);
+      }
+      if (!TAIL) tm = warp_max(tm);
+      float q[KL], sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < KL; k++) {
+        q[k] = id[k] < 0 ? 0.0f : expf(TAIL ? tv[k] : (tv[k] - tm) * a.inv_t);
+        sum += q[k];
+      }
+      sum = warp_sum(sum);
+      const float inv = TAIL ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+      for (int k = 0; k < KL; k++) {
+        const int j = k * 32 + lane;
+        if (j < a.K) {
+          s_id[j] = id[k];
+          s_q[j] = s_qv[j] = q[k] * inv;
+          s_z[j] = zk[k];
+        }
+      }
+      __syncwarp();
+      // entries naming one token add up; the first of them stands for it
+#pragma unroll
+      for (int k = 0; k < KL; k++) {
+        const int j = k * 32 + lane;
+        if (k * 32 < a.K) {
+          bool again = false;
+          for (int i = 0; i < a.K; i++) again |= s_id[i] == id[k] && i != j;
+          if (id[k] < 0) {
+            if (j < a.K) s_qv[j] = -1.0f;
+          } else if (again) {
+            float qv = 0.0f;
+            bool first = true;
+            for (int i = 0; i < a.K; i++)
+              if (s_id[i] == id[k]) {
+                qv += s_q[i];
+                first = first && i >= j;
+              }
+            s_qv[j] = first ? qv : -1.0f;
           }
-        x[i] = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+      }
+      if (lane == 0) {
+        float Q = TAIL || sum == 0.0f ? sum : 1.0f;
+        if (!(sum < INFINITY)) Q = NAN;          // a NaN or +inf among the values
+        const float qr = TAIL ? 1.0f - Q : 0.0f;
+        s_sum[flip][0] = Q;
+        s_sum[flip][1] = qr < TAIL_MIN ? 0.0f : qr;            // NaN stays
+      }
+      if (TAIL) {
+        pipe.wait(t, sh);
+#pragma unroll
+        for (int k = 0; k < KL; k++) {
+          const int at = id[k] + r.mis - sh.c0 * EV;           // element of the share
+          if (id[k] >= 0 && at >= 0 && at < cnt * EV) reinterpret_cast<T *>(st)[at] = Elem<T>::none();
+        }
+        tc::fence_proxy_async();                 // a later copy into this stage comes after these writes
       }
     }
-  }
-  // ---- the row's statistics (with a tail: those of the tokens not named)
-  Part p = warp_part<T, TH, false>(x, cnt, lane_max_of<T, TH>(x, cnt), a.c);
-  if (lane == 0) s_part[warp] = p;
-  __syncthreads();
-  // entries naming one token add up; the first of them stands for it
-  for (int j = tid; j < a.K; j += TH) {
-    const int id = s_id[j];
-    float qv = 0.0f;
-    bool first = id >= 0;
-    for (int i = 0; i < a.K; i++)
-      if (s_id[i] == id) {
-        qv += s_q[i];
-        first = first && i >= j;
+    if (!TAIL || warp != 0) pipe.wait(t, sh);
+    if (TAIL) __syncthreads();
+    // ---- the row's statistics (with a tail: those of the tokens not named)
+    Part p = warp_part<T, false>(st, cnt, thread_max<T>(st, cnt), a.c);
+    if (lane == 0) s_part[flip][warp] = p;
+    if (CL) meet<false>(s_part[flip], s_from[flip], 0, a.c);
+    else __syncthreads();
+    p = join_all<false>(CL ? s_from[flip] : s_part[flip], CL ? S : TH >> 5, a.c);
+    const float Q = s_sum[flip][0], qr = s_sum[flip][1];
+    float m = p.m, all = p.s, f = 1.0f;          // e of the row is relative to p.m, times f to m
+    if (TAIL) {
+      for (int j = lane; j < a.K; j += 32) m = fmaxf(m, s_z[j]);
+      m = warp_max(m);
+      float named = 0.0f;
+      for (int j = lane; j < a.K; j += 32)
+        if (!(s_qv[j] < 0.0f)) named += exp2_fast((s_z[j] - m) * a.c);
+      f = exp2_fast(bounded((p.m - m) * a.c));
+      all = fmaf(p.s, f, warp_sum(named));
+    }
+    const float total = Q + qr;
+    if (rank == 0 && warp == 0 && (a.loss || a.loss64)) {
+      const float ls = logf(all);
+      float L = 0.0f;
+      for (int j = lane; j < a.K; j += 32) {
+        const float qv = s_qv[j];
+        if (qv > 0.0f) L += qv * (logf(qv) - ((s_z[j] - m) * a.inv_t - ls));
       }
-    s_qv[j] = first ? qv : -1.0f;
-  }
-  p = join_row<CL, W, false>(s_part, s_from, 0.0f, a.c);
-  const float Q = s_sum[0], qr = s_sum[1];
-  float m = p.m, all = p.s, f = 1.0f;            // e of the row is relative to p.m, times f to m
-  float qv[KL], zj[KL];
+      L = warp_sum(L);
+      if (TAIL && qr > 0.0f) L += qr * (logf(qr) - (logf(p.s) + (p.m - m) * a.inv_t - ls));
+      if (all == 0.0f) L = total > 0.0f ? INFINITY : 0.0f;     // a student that allows no token
+      if (all != all || total != total) L = NAN;
+      L *= w;
+      if (lane == 0) {
+        if (a.loss) a.loss[n] = L;
+        if (a.loss64) a.loss64[n] = (double)L;
+      }
+    }
+    const float g = w * a.scale * a.inv_t;
+    if (a.dz) {
+      const float coef =
+          all == 0.0f ? 0.0f : g * (total * f / all - (TAIL && qr > 0.0f && p.s > 0.0f ? qr / p.s : 0.0f));
+      const f32x2 nm2 = pack2(-p.m, -p.m), c2 = pack2(a.c, a.c), k2 = pack2(coef, coef);
+#pragma unroll 4
+      for (int i = tid; i < cnt; i += TH) {
+        float v[EV];
+        Elem<T>::unpack(st[i], v);
 #pragma unroll
-  for (int k = 0; k < KL; k++) {
-    const int j = k * 32 + lane;
-    qv[k] = j < a.K ? s_qv[j] : -1.0f;
-    zj[k] = j < a.K ? s_z[j] : -INFINITY;
-  }
-  if (TAIL) {
-#pragma unroll
-    for (int k = 0; k < KL; k++) m = fmaxf(m, zj[k]);
-    m = warp_max(m);
-    float named = 0.0f;
-#pragma unroll
-    for (int k = 0; k < KL; k++)
-      if (!(qv[k] < 0.0f)) named += exp2_fast((zj[k] - m) * a.c);
-    f = exp2_fast(bounded((p.m - m) * a.c));
-    all = fmaf(p.s, f, warp_sum(named));
-  }
-  const float ls = logf(all);
-  const float total = Q + qr;
-  if (rank == 0 && warp == 0 && (a.loss || a.loss64)) {
-    float L = 0.0f;
-#pragma unroll
-    for (int k = 0; k < KL; k++)
-      if (qv[k] > 0.0f) L += qv[k] * (logf(qv[k]) - ((zj[k] - m) * a.inv_t - ls));
-    L = warp_sum(L);
-    if (TAIL && qr > 0.0f) L += qr * (logf(qr) - (logf(p.s) + (p.m - m) * a.inv_t - ls));
-    if (all == 0.0f) L = total > 0.0f ? INFINITY : 0.0f;       // a student that allows no token
-    if (all != all || total != total) L = NAN;
-    L *= w;
-    if (lane == 0) {
-      if (a.loss) a.loss[n] = L;
-      if (a.loss64) a.loss64[n] = (double)L;
+        for (int e = 0; e < EV; e += 2) {
+          float d0, d1;
+          unpack2(mul2(add2(pack2(v[e], v[e + 1]), nm2), c2), d0, d1);
+          unpack2(mul2(pack2(exp2_fast(d0), exp2_fast(d1)), k2), v[e], v[e + 1]);
+        }
+        store(sh.c0 + i, v);
+      }
+    }
+    __syncthreads();
+    if (tid == 0 && ahead < N) pipe.issue(t, ahead, pipe.at, next_counts);
+    pipe.next();
+    if (!a.dz || all == 0.0f) continue;
+    for (int j = tid; j < a.K; j += TH) {
+      const float q = s_qv[j];
+      if (q < 0.0f) continue;
+      const int id = s_id[j], at = (id + r.mis) / EV;
+      if (at < sh.c0 || at >= sh.c0 + cnt) continue;   // another block's
+      const float pv = exp2_fast((s_z[j] - m) * a.c) / all;
+      o.row[id] = Elem<T>::from_f(g * (total * pv - q));
     }
   }
-  if (!a.dz) return;
-  const float g = w * a.scale * a.inv_t;
-  const float coef = all == 0.0f ? 0.0f : g * (total * f / all - (TAIL && qr > 0.0f && p.s > 0.0f ? qr / p.s : 0.0f));
-  const f32x2 nm2 = pack2(-p.m, -p.m), c2 = pack2(a.c, a.c), k2 = pack2(coef, coef);
-#pragma unroll
-  for (int i = 0; i < NV; i++) {
-    const int c = c0 + i * TH + tid;
-    if (c >= c1) break;
-    float v[EV];
-    Elem<T>::unpack(x[i], v);
-#pragma unroll
-    for (int e = 0; e < EV; e += 2) {
-      float d0, d1;
-      unpack2(mul2(add2(pack2(v[e], v[e + 1]), nm2), c2), d0, d1);
-      unpack2(mul2(pack2(exp2_fast(d0), exp2_fast(d1)), k2), v[e], v[e + 1]);
-    }
-    store(c, v);
-  }
-  if (all == 0.0f) return;
-  __syncthreads();
-  for (int j = tid; j < a.K; j += TH) {
-    const float q = s_qv[j];
-    if (q < 0.0f) continue;
-    const int id = s_id[j], at = (id + r.mis) / EV;
-    if (at < c0 || at >= c1) continue;           // another block's
-    const float pv = exp2_fast((s_z[j] - m) * a.c) / all;
-    o.row[id] = Elem<T>::from_f(g * (total * pv - q));
-  }
+  if (CL) TM::sync();                            // no block leaves while another may write to it
 }
 
 }  // namespace lg
@@ -353,26 +358,13 @@ template <typename T> int grad_typed(DeviceCtx *c, const lg::GradArgs &a) {
   return launch_grad<T, 256>(c, nch, a);
 }
 
-template <typename T, int TH, bool CL, bool TAIL>
-int launch_distill(DeviceCtx *c, int N, int S, const lg::DistillArgs &a) {
-  if constexpr (!CL) {
-    lg::distill_kernel<T, TH, false, TAIL><<<N, TH, 0, c->stream>>>(a);
-    TL_TRY_CUDA(cudaGetLastError());
-    return TL_OK;
-  } else {
-    return launch_rows_cluster((const void *)lg::distill_kernel<T, TH, true, TAIL>, c, N, TH, S, const_cast<void *>(static_cast<const void *>(&a)));
-  }
+template <typename T, bool CL, bool TAIL> int launch_distill(DeviceCtx *c, const RowPlan &pl, lg::DistillArgs a) {
+  static Resident seen[kMaxDevices];
+  return launch_rows((const void *)lg::distill_kernel<T, CL, TAIL>, c, pl, 32 * a.K, &seen[c->device], &a);
 }
-template <typename T, bool TAIL> int distill_typed(DeviceCtx *c, int N, const RowPlan &pl, const lg::DistillArgs &a) {
-  if (pl.blocks > 1)
-    return pl.threads == 256 ? launch_distill<T, 256, true, TAIL>(c, N, pl.blocks, a)
-                             : launch_distill<T, 512, true, TAIL>(c, N, pl.blocks, a);
-  switch (pl.threads) {
-    case 32: return launch_distill<T, 32, false, TAIL>(c, N, 1, a);
-    case 128: return launch_distill<T, 128, false, TAIL>(c, N, 1, a);
-    case 256: return launch_distill<T, 256, false, TAIL>(c, N, 1, a);
-    default: return launch_distill<T, 512, false, TAIL>(c, N, 1, a);
-  }
+template <typename T> int distill_typed(DeviceCtx *c, const RowPlan &pl, const lg::DistillArgs &a, bool tail) {
+  if (pl.blocks > 1) return tail ? launch_distill<T, true, true>(c, pl, a) : launch_distill<T, true, false>(c, pl, a);
+  return tail ? launch_distill<T, false, true>(c, pl, a) : launch_distill<T, false, false>(c, pl, a);
 }
 
 }  // namespace
@@ -393,12 +385,11 @@ int k_distill_topk(DeviceCtx *c, const LogitRows &z, const int *t_ids, const flo
                    void *dlogits, long long ldd) {
   TraceScope ts(c, "k_distill_topk");
   const RowPlan pl = plan_rows(c, z, 0);
-  const lg::DistillArgs a{z.p, z.ld, t_ids, t_vals, K, z.V, lg::LOG2E / temperature, 1.0f / temperature, weight,
-                          scale, loss, loss64, dlogits, ldd, c->err_flag};
-  if (z.dtype == TL_F32) return tail ? distill_typed<float, true>(c, z.N, pl, a) : distill_typed<float, false>(c, z.N, pl, a);
-  if (z.dtype == TL_BF16)
-    return tail ? distill_typed<__nv_bfloat16, true>(c, z.N, pl, a) : distill_typed<__nv_bfloat16, false>(c, z.N, pl, a);
-  return tail ? distill_typed<__half, true>(c, z.N, pl, a) : distill_typed<__half, false>(c, z.N, pl, a);
+  const lg::DistillArgs a{pl.l, t_ids, t_vals, K, lg::LOG2E / temperature, 1.0f / temperature, weight, scale, loss,
+                          loss64, dlogits, ldd, c->err_flag};
+  if (z.dtype == TL_F32) return distill_typed<float>(c, pl, a, tail);
+  if (z.dtype == TL_BF16) return distill_typed<__nv_bfloat16>(c, pl, a, tail);
+  return distill_typed<__half>(c, pl, a, tail);
 }
 
 }  // namespace tl

@@ -1,18 +1,19 @@
 // tl_logits_score.cu -- log probability of a given token a row, the row's
 // entropy and its most likely tokens in one pass over the logits.
 //
-// A row's slice is loaded once and stays in registers: its largest logit, the
-// sums of e and e d relative to it, and the alternatives all come from there.
-//
 // The K most likely tokens.  A threshold below the K-th largest logit is found
-// without sorting the row: each full warp of the row's F takes the j-th
-// largest of its 32 lanes' maxima, j = ceil(K / F), and the threshold is the
-// least of these.  Each of the F warps has j elements at or above it, so there
-// are K.  About 1.5 K of random logits pass; they are collected in the first
+// without sorting the row.  Of the row's F full warps each takes the j-th
+// largest of its 32 lanes' maxima, j about 5/4 K / F; each block takes the
+// g-th largest of its F_b full warps' values, g = K F_b / (j F) rounded up;
+// the threshold is the least of the blocks'.  Every one of the g warps has j
+// elements at or above it, so the row has at least j sum g >= K.  Of random
+// logits 1.5 to 2 K pass (5/4: with j = 1 and all warps counted it is up to
+// 4.5 K, the least of many maxima being low).  They are collected in the first
 // block's shared memory as 64-bit keys (logit, then the lower index), and each
 // one's place is the number of larger keys.  Where more pass than the memory
-// holds (many equal logits, sorted rows) the K-th largest key is found by
-// bisection, counting over the registers, and exactly K are collected.
+// holds (many equal logits, rows in order) the K-th largest key is found by
+// bisection, counting over the share, and exactly K are collected.
+#include <algorithm>
 #include <cmath>
 #include "tl_logits_dev.cuh"
 #include "tl_trace.cuh"
@@ -36,43 +37,27 @@ __device__ __forceinline__ float value_of(unsigned long long key) {
   return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
 }
 
-// The j-th largest of the lanes' values (1 <= j <= 32): a bitonic sort of the
-// warp in descending order.
-__device__ __forceinline__ float warp_nth_largest(float v, int j) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int k = 2; k <= 32; k <<= 1)
-#pragma unroll
-    for (int o = k >> 1; o; o >>= 1) {
-      const float u = __shfl_xor_sync(FULL, v, o);
-      v = ((lane & o) == 0) == ((lane & k) == 0) ? fmaxf(v, u) : fminf(v, u);
-    }
-  return __shfl_sync(FULL, v, j - 1);
-}
-
 // The K largest keys of the row into the first block's memory, by bisection:
-// the thread's chunks x (the first holding element v0, the next TH chunks
-// on), at least K of them at or above thr > -inf or thr = -inf.  Every thread
-// of the row's blocks calls it.  Kept out of line, its chunks in local memory:
-// it takes 2 to 50 counting passes of about a microsecond, on rows with many
-// equal logits or of sorted order.
-template <typename T, int TH, bool CL>
-__device__ __noinline__ void select_exactly(const uint4 *x, int v0, int V, int K, float thr, unsigned *s_count,
-                                            unsigned long long *s_keys) {
+// at least K logits are at or above thr, or thr = -inf.  `first` is the share's
+// first element.  Every thread of the row's blocks calls it.  2 to 50 counting
+// passes over shared memory, of about a microsecond each.
+template <typename T, bool CL>
+__device__ __noinline__ void select_exactly(const uint4 *st, int cnt, int first, int V, int K, float thr,
+                                            unsigned *s_count, unsigned long long *s_keys) {
   using TM = Team<CL>;
-  constexpr int W = TH / 32, EV = Elem<T>::EV;
-  __shared__ int s_cnt[2][W], s_sum[2][MAX_CLUSTER];
-  const int tid = threadIdx.x;
+  constexpr int EV = Elem<T>::EV;
+  __shared__ int s_cnt[2][MAX_WARPS], s_sum[2][MAX_CLUSTER];
+  const int tid = threadIdx.x, TH = blockDim.x, W = TH >> 5;
   const unsigned S = TM::size();
   int flip = 0;
   // elements of an order above u, and those of order u and an index below b
   auto count = [&](unsigned u, int b) {
     int k = 0;
 #pragma unroll 1
-    for (int i = 0; i < NV; i++) {
+    for (int i = tid; i < cnt; i += TH) {
       float f[EV];
-      Elem<T>::unpack(x[i], f);
-      const int v = v0 + i * TH * EV;
+      Elem<T>::unpack(st[i], f);
+      const int v = first + i * EV;
 #pragma unroll
       for (int e = 0; e < EV; e++) {
         const unsigned o = order_of(f[e]);
@@ -114,10 +99,10 @@ __device__ __noinline__ void select_exactly(const uint4 *x, int v0, int V, int K
   unsigned *to = TM::at(s_count, 0);
   unsigned long long *keys = TM::at(s_keys, 0);
 #pragma unroll 1
-  for (int i = 0; i < NV; i++) {
+  for (int i = tid; i < cnt; i += TH) {
     float f[EV];
-    Elem<T>::unpack(x[i], f);
-    const int v = v0 + i * TH * EV;
+    Elem<T>::unpack(st[i], f);
+    const int v = first + i * EV;
 #pragma unroll
     for (int e = 0; e < EV; e++) {
       const unsigned o = order_of(f[e]);
@@ -130,151 +115,224 @@ __device__ __noinline__ void select_exactly(const uint4 *x, int v0, int V, int K
   TM::sync();
 }
 
+// Keys in descending order, four a lane (lane l holds places 4l .. 4l + 3): a
+// bitonic sort of 128 in one warp.
+__device__ __forceinline__ void sort_128(unsigned long long (&k)[4]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int size = 2; size <= 128; size <<= 1)
+#pragma unroll
+    for (int o = size >> 1; o; o >>= 1)
+      if (o >= 4) {
+        const bool larger = ((lane * 4 & o) == 0) == ((lane * 4 & size) == 0);
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const unsigned long long u = __shfl_xor_sync(FULL, k[r], o >> 2);
+          k[r] = (u > k[r]) == larger ? u : k[r];
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+          if (!(r & o)) {
+            const bool down = ((lane * 4 + r) & size) == 0;
+            const unsigned long long x = k[r], y = k[r | o];
+            const bool swap = (y > x) == down;
+            k[r] = swap ? y : x;
+            k[r | o] = swap ? x : y;
+          }
+      }
+}
+
 struct ScoreArgs {
-  const void *z;
-  long long ld;
+  Layout l;
   const int *ids;
-  int V;
   float c, inv_t;                    // log2(e) / temperature, 1 / temperature
   float *logp, *entropy, *stats;
-  int K;
+  int K, j, g_full;                  // alternatives; see threshold() for j and g_full
   int *top_ids;
   float *top_logp;
   int *err;
 };
 
-template <typename T, int TH, bool CL, bool ENT>
-__global__ void __launch_bounds__(TH, 1024 / TH) score_kernel(const ScoreArgs a) {
+template <typename T, bool CL, bool ENT>
+__global__ void __launch_bounds__(MAX_THREADS, 2) score_kernel(const ScoreArgs a) {
   using TM = Team<CL>;
-  constexpr int W = TH / 32, EV = Elem<T>::EV;
-  __shared__ Part s_part[W], s_from[MAX_CLUSTER];
-  __shared__ unsigned s_count;
-  __shared__ unsigned long long s_keys[CAP];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const unsigned rank = TM::rank(), S = TM::size();
-  const size_t n = CL ? blockIdx.x / S : blockIdx.x;
-  const Chunks<T> r(static_cast<const T *>(a.z) + n * a.ld, a.V);
-  const int per = CL ? (r.n + (int)S - 1) / (int)S : r.n;
-  const int c0 = (int)rank * per, c1 = min(r.n, c0 + per), cnt = c1 - c0;
-  if (tid == 0) s_count = 0;
-  TM::arrive();
-
-  uint4 x[NV];
-  load_slice<T, TH>(r, c0, c1, x);
-  // the given token's logit, read by the thread that reports it
-  int id = -1;
-  float z_id = 0.0f;
-  if (rank == 0 && tid == 0 && a.logp) {
-    id = a.ids[n];
-    if (id >= 0 && id < a.V) {
-      z_id = Elem<T>::to_f(r.row[id]);
-    } else {
-      if (id != -1) atomicExch(a.err, 100);
-      id = -1;
-    }
+  constexpr int EV = Elem<T>::EV;
+  extern __shared__ __align__(128) unsigned char s_dyn[];
+  __shared__ Part s_part[2][MAX_WARPS], s_from[2][MAX_CLUSTER];
+  __shared__ unsigned s_count[2];
+  __shared__ uint64_t s_full[MAX_STAGES];
+  __shared__ int s_abort;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, TH = blockDim.x, W = TH >> 5;
+  const int S = (int)TM::size(), rank = (int)TM::rank();
+  const Rows<T> t(a.l, rank);
+  const int N = a.l.N, stride = (int)gridDim.x / S, first_row = (int)blockIdx.x / S;
+  unsigned long long *s_keys = reinterpret_cast<unsigned long long *>(s_dyn + (size_t)a.l.stages * a.l.chunks * 16);
+  Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), a.l.stages, a.l.chunks, s_full, &s_abort, a.err};
+  // full warps of this block, in every row: those whose 32 lanes all hold logits
+  const int mine = max(0, min(min((a.l.V + EV - 1) / EV - t.c0, t.per), TH)) >> 5;
+  const int g = a.j ? (a.K * mine + a.j * a.g_full - 1) / (a.j * a.g_full) : 0;
+  const bool reports = rank == 0 && tid == 0;    // the thread that writes a row's scalars
+  if (tid == 0) {
+    pipe.init();
+    for (int i = 0; i < a.l.stages; i++)
+      if (first_row + i * stride < N) pipe.issue(t, first_row + i * stride, i, true);
+    s_count[0] = s_count[1] = 0;
   }
-  const float lane_max = lane_max_of<T, TH>(x, cnt);
-  float thr = INFINITY;              // a warp that is not full sets none
-  if (a.K) {
-    int full = 0;                    // full warps of the row
-    for (int i = 0; i < (int)S; i++) full += min(max(min(per, r.n - i * per), 0), TH) >> 5;
-    const int j = full ? (a.K + full - 1) / full : 33;
-    if (j > 32) thr = -INFINITY;     // too few maxima: every element passes
-    else if (min(cnt, TH) >= warp * 32 + 32) thr = j == 1 ? warp_max(lane_max) : warp_nth_largest(lane_max, j);
-  }
-  Part p = warp_part<T, TH, ENT>(x, cnt, lane_max, a.c);
-  p.w = thr;
-  if (lane == 0) s_part[warp] = p;
-  p = join_row<CL, W, ENT>(s_part, s_from, INFINITY, a.c);
-  const float ls = logf(p.s);        // -inf where nothing is left, NaN for a row without a distribution
-  const bool bad = !(p.s >= 0.0f);
-  if (rank == 0 && tid == 0) {
-    if (a.logp)
-      a.logp[n] = id < 0 ? 0.0f : p.s == 0.0f ? -INFINITY : (z_id - p.m) * a.inv_t - ls;
-    if (ENT) {
-      const float h = ls - p.t / p.s * LN2;
-      a.entropy[n] = p.s == 0.0f || h < 0.0f ? 0.0f : h;
+  int id_next = reports && a.logp ? a.ids[first_row] : -1;
+  TM::sync();
+  for (int n = first_row, flip = 0; n < N; n += stride, flip ^= 1) {
+    const Share<T> sh(t, n);
+    // the given token's logit, and the next row's token
+    int id = id_next;
+    float z_id = 0.0f;
+    if (reports && a.logp) {
+      if (id >= 0 && id < t.V) {
+        z_id = Elem<T>::to_f(sh.r.row[id]);
+      } else {
+        if (id != -1) atomicExch(a.err, ERR_TOKEN);
+        id = -1;
+      }
+      if (n + stride < N) id_next = a.ids[n + stride];
     }
-    if (a.stats) {
-      a.stats[2 * n] = p.m;
-      a.stats[2 * n + 1] = p.s == 0.0f ? INFINITY : ls;
-    }
-  }
-  if (!a.K) return;
-
-  // ---- the alternatives
-  thr = p.w;
-  unsigned *count = TM::at(&s_count, 0);
-  unsigned long long *keys = TM::at(s_keys, 0);
-  if (lane_max >= thr && lane_max > -INFINITY) {
+    const int cnt = sh.cnt;
+    const uint4 *st = pipe.stage();
+    pipe.wait(t, sh);
+    const float top = thread_max<T>(st, cnt);
+    float w = -INFINITY;
+    if (a.j && warp < mine) w = a.j == 1 ? warp_max(top) : nth_largest<32>(top, a.j);
+    Part p = warp_part<T, ENT>(st, cnt, top, a.c);
+    p.w = w;
+    if (lane == 0) s_part[flip][warp] = p;
+    if (CL) meet<ENT>(s_part[flip], s_from[flip], g, a.c);
+    else __syncthreads();
+    const Part *parts = CL ? s_from[flip] : s_part[flip];
+    const int ahead = n + a.l.stages * stride;
+    if (!a.K && tid == 0 && ahead < N) pipe.issue(t, ahead, pipe.at, true);
+    unsigned found = 0;
+    if (a.K) {                       // ---- the alternatives
+      float thr = -INFINITY;         // too few maxima: every element passes
+      if (CL) {
+        if (a.j) {
+          thr = (lane & 15) < S ? parts[lane & 15].w : INFINITY;
 #pragma unroll
-    for (int i = 0; i < NV; i++)
-      if (i * TH < cnt && Elem<T>::max_of(x[i]) >= thr) {
-        float f[EV];
-        Elem<T>::unpack(x[i], f);
-        const int v = r.first(c0 + i * TH + tid);
+          for (int o = 8; o; o >>= 1) thr = fminf(thr, __shfl_xor_sync(FULL, thr, o));
+        }
+      } else if (a.j) {
+        thr = W == 1 ? parts[0].w : nth_largest<16>((lane & 15) < W ? parts[lane & 15].w : -INFINITY, g);
+      }
+      unsigned *count = TM::at(&s_count[flip], 0);
+      unsigned long long *keys = TM::at(s_keys, 0);
+      if (top >= thr && top > -INFINITY) {
+#pragma unroll 2
+        for (int i = tid; i < cnt; i += TH) {
+          const uint4 x = st[i];
+          if (Elem<T>::max_of(x) >= thr) {
+            float f[EV];
+            Elem<T>::unpack(x, f);
+            const int v = sh.r.first(sh.c0 + i);
 #pragma unroll
-        for (int e = 0; e < EV; e++)
-          if (f[e] >= thr && f[e] > -INFINITY) {
-            const unsigned at = atomicAdd(count, 1u);
-            if (at < CAP) keys[at] = key_of(f[e], v + e);
+            for (int e = 0; e < EV; e++)
+              if (f[e] >= thr && f[e] > -INFINITY) {
+                const unsigned at = atomicAdd(count, 1u);
+                if (at < CAP) keys[at] = key_of(f[e], v + e);
+              }
+          }
+        }
+      }
+      TM::sync();
+      found = *count;
+      if (found > CAP) {
+        const Part all = join_all<false>(parts, CL ? S : W, a.c);
+        if (all.s >= 0.0f) {         // a row without a distribution has no alternatives
+          select_exactly<T, CL>(st, cnt, sh.r.first(sh.c0), t.V, a.K, thr, &s_count[flip], s_keys);
+          found = *count;
+        }
+      }
+      if (tid == 0 && ahead < N) pipe.issue(t, ahead, pipe.at, true);
+    }
+    // ---- results: the first block's first warp, and all its warps where many
+    // candidates are left to put in order
+    const bool crowd = found > 128;
+    if (rank == 0 && (warp == 0 || crowd)) {
+      p = join_all<ENT>(parts, CL ? S : W, a.c);
+      const float ls = logf(p.s);    // -inf where nothing is left, NaN for a row without a distribution
+      const bool bad = !(p.s >= 0.0f);
+      if (tid == 0) {
+        s_count[flip ^ 1] = 0;       // its readers have passed a barrier of this row
+        if (a.logp) a.logp[n] = id < 0 ? 0.0f : p.s == 0.0f ? -INFINITY : (z_id - p.m) * a.inv_t - ls;
+        if (ENT) {
+          const float h = ls - p.t / p.s * LN2;
+          a.entropy[n] = p.s == 0.0f || h < 0.0f ? 0.0f : h;
+        }
+        if (a.stats) {
+          a.stats[2 * (size_t)n] = p.m;
+          a.stats[2 * (size_t)n + 1] = p.s == 0.0f ? INFINITY : ls;
+        }
+      }
+      if (a.K) {
+        const int got = bad ? 0 : (int)min(found, (unsigned)CAP);
+        int *to_id = a.top_ids + (size_t)n * a.K;
+        float *to_lp = a.top_logp + (size_t)n * a.K;
+        auto put = [&](int place, unsigned long long k) {
+          if (place >= a.K) return;
+          to_id[place] = (int)(0xFFFFFFFFu - (unsigned)k);
+          to_lp[place] = (value_of(k) - p.m) * a.inv_t - ls;
+        };
+        if (crowd || got <= 24) {
+          for (int i = tid; i < got; i += crowd ? TH : 32) {
+            const unsigned long long k = s_keys[i];
+            int place = 0;
+            for (int q = 0; q < got; q++) place += s_keys[q] > k;
+            put(place, k);
+          }
+        } else {
+          unsigned long long k[4];
+#pragma unroll
+          for (int r = 0; r < 4; r++) k[r] = lane * 4 + r < got ? s_keys[lane * 4 + r] : 0;
+          sort_128(k);
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+            if (lane * 4 + r < got) put(lane * 4 + r, k[r]);
+        }
+        if (warp == 0)
+          for (int i = got + lane; i < a.K; i += 32) {
+            to_id[i] = -1;
+            to_lp[i] = bad ? NAN : -INFINITY;
           }
       }
-  }
-  TM::sync();
-  unsigned found = *count;
-  if (found > CAP && !bad) {
-    uint4 kept[NV];
-#pragma unroll
-    for (int i = 0; i < NV; i++) kept[i] = x[i];
-    select_exactly<T, TH, CL>(kept, r.first(c0 + tid), a.V, a.K, thr, &s_count, s_keys);
-    found = *count;
-  }
-  if (CL) {                          // the first block's memory has been read by all
-    TM::arrive();
-    TM::wait();
-  }
-  if (rank != 0) return;
-  const int got = bad ? 0 : (int)min(found, (unsigned)CAP);
-  for (int i = tid; i < got; i += TH) {
-    const unsigned long long k = s_keys[i];
-    int place = 0;
-    for (int j = 0; j < got; j++) place += s_keys[j] > k;
-    if (place < a.K) {
-      a.top_ids[n * a.K + place] = (int)(0xFFFFFFFFu - (unsigned)k);
-      a.top_logp[n * a.K + place] = (value_of(k) - p.m) * a.inv_t - ls;
     }
+    pipe.next();
   }
-  for (int i = got + tid; i < a.K; i += TH) {
-    a.top_ids[n * a.K + i] = -1;
-    a.top_logp[n * a.K + i] = bad ? NAN : -INFINITY;
-  }
+  if (CL) TM::sync();                // the first block's memory stays until all have read it
 }
 
 }  // namespace lg
 
 namespace {
 
-template <typename T, int TH, bool CL, bool ENT>
-int launch_score(DeviceCtx *c, int N, int S, const lg::ScoreArgs &a) {
-  if constexpr (!CL) {
-    lg::score_kernel<T, TH, false, ENT><<<N, TH, 0, c->stream>>>(a);
-    TL_TRY_CUDA(cudaGetLastError());
-    return TL_OK;
-  } else {
-    return launch_rows_cluster((const void *)lg::score_kernel<T, TH, true, ENT>, c, N, TH, S, const_cast<void *>(static_cast<const void *>(&a)));
-  }
+template <typename T, bool CL, bool ENT> int launch_score(DeviceCtx *c, const RowPlan &pl, lg::ScoreArgs a) {
+  static Resident seen[kMaxDevices];
+  return launch_rows((const void *)lg::score_kernel<T, CL, ENT>, c, pl, a.K ? lg::CAP * 8 : 0, &seen[c->device], &a);
 }
-template <typename T, bool ENT> int score_typed(DeviceCtx *c, int N, const RowPlan &pl, const lg::ScoreArgs &a) {
-  if (pl.blocks > 1)
-    return pl.threads == 256 ? launch_score<T, 256, true, ENT>(c, N, pl.blocks, a)
-                             : launch_score<T, 512, true, ENT>(c, N, pl.blocks, a);
-  switch (pl.threads) {
-    case 32: return launch_score<T, 32, false, ENT>(c, N, 1, a);
-    case 128: return launch_score<T, 128, false, ENT>(c, N, 1, a);
-    case 256: return launch_score<T, 256, false, ENT>(c, N, 1, a);
-    default: return launch_score<T, 512, false, ENT>(c, N, 1, a);
-  }
+template <typename T> int score_typed(DeviceCtx *c, const RowPlan &pl, const lg::ScoreArgs &a) {
+  if (pl.blocks > 1) return a.entropy ? launch_score<T, true, true>(c, pl, a) : launch_score<T, true, false>(c, pl, a);
+  return a.entropy ? launch_score<T, false, true>(c, pl, a) : launch_score<T, false, false>(c, pl, a);
+}
+
+// What the threshold goes by: the row's full warps F (g_full) and the j of
+// "the j-th largest of a warp's 32 maxima", 0 where 32 F maxima are fewer than K.
+void threshold(const RowPlan &pl, int ev, lg::ScoreArgs *a) {
+  const int nch = (a->l.V + ev - 1) / ev;        // chunks that every row has, whatever its alignment
+  int full = 0;
+  for (int i = 0; i < pl.blocks; i++)
+    full += std::max(0, std::min(std::min(nch - i * a->l.per, a->l.per), pl.threads)) / 32;
+  a->g_full = full;
+  a->j = 0;
+  if (!a->K || !full) return;
+  a->j = (5 * a->K + 4 * full - 1) / (4 * full);
+  if (a->j > 32) a->j = (a->K + full - 1) / full;
+  if (a->j > 32) a->j = 0;
 }
 
 }  // namespace
@@ -283,12 +341,12 @@ int k_token_logprobs(DeviceCtx *c, const LogitRows &z, const int *ids, float tem
                      float *entropy, float *stats, int K, int *top_ids, float *top_logp) {
   TraceScope ts(c, "k_token_logprobs");
   const RowPlan pl = plan_rows(c, z, K);
-  const lg::ScoreArgs a{z.p, z.ld, ids, z.V, lg::LOG2E / temperature, 1.0f / temperature, logp, entropy, stats, K,
-                        top_ids, top_logp, c->err_flag};
-  if (z.dtype == TL_F32) return entropy ? score_typed<float, true>(c, z.N, pl, a) : score_typed<float, false>(c, z.N, pl, a);
-  if (z.dtype == TL_BF16)
-    return entropy ? score_typed<__nv_bfloat16, true>(c, z.N, pl, a) : score_typed<__nv_bfloat16, false>(c, z.N, pl, a);
-  return entropy ? score_typed<__half, true>(c, z.N, pl, a) : score_typed<__half, false>(c, z.N, pl, a);
+  lg::ScoreArgs a{pl.l, ids, lg::LOG2E / temperature, 1.0f / temperature, logp, entropy, stats, K, 0, 0, top_ids,
+                  top_logp, c->err_flag};
+  threshold(pl, z.dtype == TL_F32 ? 4 : 8, &a);
+  if (z.dtype == TL_F32) return score_typed<float>(c, pl, a);
+  if (z.dtype == TL_BF16) return score_typed<__nv_bfloat16>(c, pl, a);
+  return score_typed<__half>(c, pl, a);
 }
 
 }  // namespace tl
