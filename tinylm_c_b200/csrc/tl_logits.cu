@@ -19,26 +19,33 @@ RowPlan plan_rows(const DeviceCtx *c, const LogitRows &z, int K) {
   const bool one = (z.ld * es) % 16 == 0 || z.N == 1;
   const int mis = one ? (int)(reinterpret_cast<uintptr_t>(z.p) & 15) / es : ev - 1;
   const int nch = (z.V + mis + ev - 1) / ev;
-  int blocks = (nch + 2047) / 2048;
-  if (blocks > lg::MAX_CLUSTER) blocks = lg::MAX_CLUSTER;
-  // few rows: more blocks a row
-  while ((long long)z.N * blocks * 2 <= c->num_sms && blocks * 2 <= 8 && nch / blocks >= 512) blocks *= 2;
-  const int per = (nch + blocks - 1) / blocks;
-  RowPlan p{256, blocks, {z.p, z.ld, z.N, z.V, per, 2, (per + 7) / 8 * 8, 0}};
-  if (per > 2048 + 256) p.threads = 512;
-  else if (blocks == 1 && per <= 256 && K <= 16) p.threads = 32;
-  else if (per <= 1024) p.threads = 128;
-  if (p.threads == 32) p.l.stages = 4;
+  // few rows: several blocks a row
+  int blocks = 1;
+  while ((long long)z.N * blocks * 2 <= 4 * c->num_sms && blocks * 2 <= 8 && nch / blocks >= 512) blocks *= 2;
+  RowPlan p{256, blocks, {z.p, z.ld, z.N, z.V, nch, 1, 1, 0, 0}};
+  if (blocks > 1) {
+    if ((nch + blocks - 1) / blocks > 6144) blocks = p.blocks = (nch + 6143) / 6144;
+    p.l.per = (nch + blocks - 1) / blocks;
+    p.l.pieces = blocks;
+    p.threads = p.l.per <= 512 ? 128 : p.l.per <= 2048 ? 256 : 512;
+  } else {
+    p.threads = nch <= 256 && K <= 16 ? 32 : nch <= 1024 ? 128 : 256;
+    p.l.per = nch < 2048 ? nch : 2048;
+    p.l.pieces = (nch + p.l.per - 1) / p.l.per;
+    p.l.stages = p.threads == 32 ? 4 : 2;
+  }
+  p.l.chunks = (p.l.per + 7) / 8 * 8;
   p.l.ragged = !one || mis || (z.V % ev) != 0;
   return p;
 }
 
-int launch_rows(const void *kernel, DeviceCtx *c, const RowPlan &p, int more_smem, Resident *seen, void *args) {
+int launch_rows(const void *kernel, DeviceCtx *c, const RowPlan &p, int more_threads, int more_smem, Resident *seen, void *args) {
   constexpr int kMaxDynamic = 220 * 1024;          // of 227 KB a block may have, less the kernels' static part
   const int smem = p.l.stages * p.l.chunks * 16 + more_smem;
   if (smem > kMaxDynamic) return set_error(TL_EINVAL, "rows need %d bytes of shared memory a block", smem);
   cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3((unsigned)p.threads);
+  const int threads = p.threads + more_threads;
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = c->stream;
   cudaLaunchAttribute at;
@@ -56,17 +63,17 @@ int launch_rows(const void *kernel, DeviceCtx *c, const RowPlan &p, int more_sme
   }
   int fit = 0;
   for (const Resident::Shape &s : seen->of)
-    if (s.threads == p.threads && s.blocks == p.blocks && s.smem == smem) fit = s.fit;
+    if (s.threads == threads && s.blocks == p.blocks && s.smem == smem) fit = s.fit;
   if (!fit) {
     if (p.blocks == 1) {
-      TL_TRY_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, p.threads, (size_t)smem));
+      TL_TRY_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, threads, (size_t)smem));
       fit *= c->num_sms;
     } else {
       cfg.gridDim = dim3((unsigned)p.blocks);
       TL_TRY_CUDA(cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg));
     }
-    if (fit < 1) return set_error(TL_ECUDA, "%d blocks of %d threads and %d bytes do not fit", p.blocks, p.threads, smem);
-    seen->of[seen->next] = Resident::Shape{p.threads, p.blocks, smem, fit};
+    if (fit < 1) return set_error(TL_ECUDA, "%d blocks of %d threads and %d bytes do not fit", p.blocks, threads, smem);
+    seen->of[seen->next] = Resident::Shape{threads, p.blocks, smem, fit};
     seen->next = (seen->next + 1) % Resident::N;
   }
   cfg.gridDim = dim3((unsigned)((p.l.N < fit ? p.l.N : fit) * p.blocks));

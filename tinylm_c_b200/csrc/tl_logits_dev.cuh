@@ -29,7 +29,9 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr unsigned FULL = 0xFFFFFFFFu;
 constexpr int MAX_CLUSTER = 16;
-constexpr int MAX_THREADS = 512, MAX_WARPS = MAX_THREADS / 32, MAX_STAGES = 4;
+constexpr int MAX_WARPS = 16, MAX_STAGES = 4;
+// Blocks of TH threads an SM holds at least: 64 registers a thread.
+constexpr int min_blocks(int TH) { return 1024 / TH; }
 constexpr int ERR_COPY = 90;                       // error word: a bulk copy did not arrive in time
 constexpr int ERR_TOKEN = 100;                     // a token id outside [0, V)
 
@@ -83,6 +85,18 @@ __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
   return v;
+}
+
+// 16 bytes of shared memory at a 32-bit address.
+__device__ __forceinline__ uint4 lds(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+
+// A barrier of the TH computing threads of a block that has other warps too.
+template <int TH> __device__ __forceinline__ void bar_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(TH) : "memory");
 }
 
 // ------------------------------------------------------------ element types
@@ -200,121 +214,114 @@ template <typename T> struct Chunks {
       }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  __device__ __forceinline__ void store_each(int c, const float (&f)[EV]) const {
-    const int v = first(c);
-#pragma unroll
-    for (int e = 0; e < EV; e++)
-      if (v + e >= 0 && v + e < V) row[v + e] = Elem<T>::from_f(f[e]);
-  }
 };
 
-// The tensor's rows and how they are shared out, as the host lays it out: each
-// of a row's blocks has `per` chunks (the last one what is left) and `stages`
-// buffers of `chunks` >= per chunks; `ragged`: some row's ends do not fill
-// their chunks.
+// The tensor's rows and how they are cut up, as the host lays it out: into
+// pieces of `per` chunks, one for each block of a row's cluster or, one after
+// another, for the one block that has the row (`pieces` of them, the last with
+// what is left); each block has `stages` buffers of `chunks` >= per chunks.
+// `ragged`: some row's ends do not fill their chunks.
 struct Layout {
   const void *z;
   long long ld;
-  int N, V, per, stages, chunks, ragged;
+  int N, V, per, pieces, stages, chunks, ragged;
 };
 template <typename T> struct Rows {
   const T *z;
   long long ld;
-  int V, c0, per;
+  int V, per;
   uintptr_t end;                       // one past the last row
   bool ragged;
-  __device__ __forceinline__ Rows(const Layout &l, int rank)
-      : z(static_cast<const T *>(l.z)), ld(l.ld), V(l.V), c0(rank * l.per), per(l.per),
+  __device__ __forceinline__ explicit Rows(const Layout &l)
+      : z(static_cast<const T *>(l.z)), ld(l.ld), V(l.V), per(l.per),
         end(reinterpret_cast<uintptr_t>(z + ((long long)(l.N - 1) * ld + V))), ragged(l.ragged) {}
+  __device__ __forceinline__ Chunks<T> row(int n) const { return Chunks<T>(z + (size_t)n * ld, V); }
+  // Whether a chunk lies inside the tensor as a whole, so that it may be copied.
+  __device__ __forceinline__ bool inside(const uint4 *p) const {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+    return a >= reinterpret_cast<uintptr_t>(z) && a + 16 <= end;
+  }
 };
-// A block's share of a row: chunks [c0, c0 + cnt), in shared memory from 0.
-template <typename T> struct Share {
+// A piece of a row: chunks [c0, c0 + cnt), in shared memory from 0.
+template <typename T> struct Piece {
   Chunks<T> r;
   int c0, cnt;
-  __device__ __forceinline__ Share(const Rows<T> &t, int n) : r(t.z + (size_t)n * t.ld, t.V) {
-    c0 = t.c0;
+  __device__ __forceinline__ Piece(const Rows<T> &t, int n, int i) : r(t.row(n)), c0(i * t.per) {
     cnt = max(0, min(r.n - c0, t.per));
   }
-  // Whether a chunk lies inside the tensor as a whole, so that it may be copied.
-  static __device__ __forceinline__ bool inside(const Rows<T> &t, const uint4 *p) {
-    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
-    return a >= reinterpret_cast<uintptr_t>(t.z) && a + 16 <= t.end;
-  }
-};
-
-// Rows on their way into `stages` buffers of `bytes` each (a multiple of 128).
-// One thread issues the copies; all wait for them.
-template <typename T> struct Pipe {
-  uint4 *buf;                          // stage 0
-  int stages, stage_chunks;
-  uint64_t *full;                      // a barrier a stage
-  int *abort_flag;                     // a copy did not arrive: nothing is waited for or copied any more
-  int *err;
-  int at = 0, phase = 0;               // the stage of the row at hand, its barrier's parity
-  __device__ __forceinline__ void init() {
-    for (int i = 0; i < stages; i++) tc::mbar_init(tc::smem_u32(&full[i]), 1);
-    *abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  __device__ __forceinline__ uint4 *stage() const { return buf + (size_t)at * stage_chunks; }
-  __device__ __forceinline__ void next() {
-    if (++at == stages) { at = 0; phase ^= 1; }
-  }
-  // Row n's share into stage s (`read` false: nothing is copied, the stage is
-  // full at once).  The stage's earlier readers have passed a barrier.  The
-  // tensor's first and last chunk, where it does not fill them, are written
-  // by the calling thread.
-  __device__ __forceinline__ void issue(const Rows<T> &t, int n, int s, bool read) const {
-    const uint32_t bar = tc::smem_u32(&full[s]);
-    if (*(volatile int *)abort_flag) return;
-    int lo = 0, hi = 0, c0 = 0;
-    const uint4 *base = nullptr;
-    if (read) {
-      const Share<T> sh(t, n);
-      base = sh.r.base;
-      c0 = lo = sh.c0;
-      hi = sh.c0 + sh.cnt;
-      uint4 *st = buf + (size_t)s * stage_chunks;
-      if (lo < hi && !Share<T>::inside(t, base + lo)) {
-        st[0] = sh.r.load_edge(lo);
-        lo++;
-      }
-      if (lo < hi && !Share<T>::inside(t, base + hi - 1)) {
-        hi--;
-        st[hi - c0] = sh.r.load_edge(hi);
-      }
-    }
-    const uint32_t bytes = (uint32_t)(hi - lo) * 16u;
-    // what other threads read of the stage comes before what the copy writes
-    tc::fence_proxy_async();
-    tc::mbar_arrive_expect_tx(bar, bytes);
-    if (bytes)
-      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                       tc::smem_u32(buf + (size_t)s * stage_chunks + (lo - c0))),
-                   "l"(__cvta_generic_to_global(base + lo)), "r"(bytes), "r"(bar)
-                   : "memory");
-  }
-  // The row at hand is in shared memory, its ends masked; the thread that
-  // reads an end chunk (t of n threads reads chunks t, t + n, ...) masks it.
-  // After an expired wait the kernel runs on over what there is, its copies
-  // and waits over, and the error word says so: leaving would strand the
-  // other blocks of the row.
-  __device__ __forceinline__ void wait(const Rows<T> &t, const Share<T> &sh) const {
-    tc::mbar_wait(tc::smem_u32(&full[at]), phase, abort_flag, err, ERR_COPY);
-    if (!t.ragged) return;
-    uint4 *st = stage();
+  // The copied elements of other rows in the row's first and last chunk set
+  // to -inf, by the thread for whom `mine(chunk of the piece)`.
+  template <typename F> __device__ __forceinline__ void mask_ends(uint4 *st, F &&mine) const {
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-      const int c = k ? sh.r.n - 1 : 0;
-      const bool partial = k ? sh.r.full1 < sh.r.n && (sh.r.n > 1 || sh.r.full0 == 0) : sh.r.full0 == 1;
-      if (partial && c >= sh.c0 && c < sh.c0 + sh.cnt && (c - sh.c0) % (int)blockDim.x == (int)threadIdx.x) {
-        T *e = reinterpret_cast<T *>(st + (c - sh.c0));
-        const int v = sh.r.first(c);
+      const int c = k ? r.n - 1 : 0;
+      const bool partial = k ? r.full1 < r.n && (r.n > 1 || r.full0 == 0) : r.full0 == 1;
+      if (partial && c >= c0 && c < c0 + cnt && mine(c - c0)) {
+        T *e = reinterpret_cast<T *>(st + (c - c0));
+        const int v = r.first(c);
         for (int i = 0; i < Elem<T>::EV; i++)
-          if (v + i < 0 || v + i >= sh.r.V) e[i] = Elem<T>::none();
+          if (v + i < 0 || v + i >= r.V) e[i] = Elem<T>::none();
         tc::fence_proxy_async();       // a later copy into this stage comes after these writes
       }
     }
+  }
+};
+
+// The stages of a block and their barriers.
+template <typename T> struct Pipe {
+  uint4 *buf;                          // stage 0
+  int stages, stage_chunks;
+  uint64_t *full;                      // a barrier a stage: a piece has arrived
+  int *abort_flag;                     // a wait ran out: nothing is waited for or copied any more
+  int *err;
+  __device__ __forceinline__ uint4 *stage(int s) const { return buf + (size_t)s * stage_chunks; }
+  // Piece p into stage s (`read` false: nothing is copied, the stage is full
+  // at once), by one thread.  The stage's earlier readers are done.  The
+  // tensor's first and last chunk, where it does not fill them, are written
+  // by the calling thread.
+  __device__ __forceinline__ void issue(const Rows<T> &t, int n, int piece, int s, bool read) const {
+    const uint32_t bar = tc::smem_u32(&full[s]);
+    if (*(volatile int *)abort_flag) return;
+    int lo = 0, hi = 0;
+    const uint4 *from = nullptr;
+    uint4 *st = stage(s);
+    // what other threads read and wrote of the stage comes before the copy
+    tc::fence_proxy_async();
+    if (read) {
+      const Piece<T> p(t, n, piece);
+      from = p.r.base + p.c0;
+      hi = p.cnt;
+      if (lo < hi && !t.inside(from)) {
+        st[0] = p.r.load_edge(p.c0);
+        lo++;
+      }
+      if (lo < hi && !t.inside(from + hi - 1)) {
+        hi--;
+        st[hi] = p.r.load_edge(p.c0 + hi);
+      }
+    }
+    const uint32_t bytes = (uint32_t)(hi - lo) * 16u;
+    tc::mbar_arrive_expect_tx(bar, bytes);
+    if (bytes)
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                       tc::smem_u32(st + lo)),
+                   "l"(__cvta_generic_to_global(from + lo)), "r"(bytes), "r"(bar)
+                   : "memory");
+  }
+  // Waits for a phase of a barrier, for two seconds at most.  After an expired
+  // wait the kernel runs on over what there is, its copies and waits over, and
+  // the error word says so: leaving would strand the other threads and blocks
+  // that meet this one.
+  __device__ __forceinline__ void wait(uint64_t *bar, uint32_t parity) const {
+    tc::mbar_wait(tc::smem_u32(bar), parity, abort_flag, err, ERR_COPY);
+  }
+};
+// Stage and phase of the k-th piece through a pipe.
+struct Turn {
+  int s = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++s == stages) { s = 0; phase ^= 1; }
   }
 };
 
@@ -359,62 +366,90 @@ template <int N> __device__ __forceinline__ float nth_largest(float v, int j) {
   return __shfl_sync(FULL, v, j - 1);
 }
 
-// This thread's largest logit of the share (-inf if it has none).
-template <typename T> __device__ __forceinline__ float thread_max(const uint4 *st, int cnt) {
-  float m = -INFINITY;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < cnt; i += blockDim.x) m = fmaxf(m, Elem<T>::max_of(st[i]));
-  return m;
-}
-// A warp's part of the row; `top` is this thread's largest logit.
-template <typename T, bool ENT>
-__device__ __forceinline__ Part warp_part(const uint4 *st, int cnt, float top, float c) {
-  constexpr int EV = Elem<T>::EV;
-  const float m = fmaxf(warp_max(top), -FLT_MAX);
-  const f32x2 nm = pack2(-m, -m), cc = pack2(c, c);
-  f32x2 s2 = pack2(0.0f, 0.0f), t2 = s2;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < cnt; i += blockDim.x) {
-    float f[EV];
-    Elem<T>::unpack(st[i], f);
-#pragma unroll
-    for (int e = 0; e < EV; e += 2) {
-      const f32x2 d = mul2(add2(pack2(f[e], f[e + 1]), nm), cc);
-      float d0, d1;
-      unpack2(d, d0, d1);
-      const f32x2 ex = pack2(exp2_fast(d0), exp2_fast(d1));
-      s2 = add2(s2, ex);
-      if (ENT) t2 = fma2(ex, pack2(bounded(d0), bounded(d1)), t2);
-    }
+// f(chunks, index of the first) for this thread's chunks tid, tid + TH, ... of
+// a share in shared memory, four at a time while four are left, then one.
+template <int TH, typename F4, typename F1>
+__device__ __forceinline__ void for_chunks(uint32_t st, int cnt, F4 &&f4, F1 &&f1) {
+  int i = threadIdx.x;
+  uint32_t at = st + 16u * threadIdx.x;
+  for (; i + 3 * TH < cnt; i += 4 * TH, at += 64u * TH) {
+    const uint4 x[4] = {lds(at), lds(at + 16 * TH), lds(at + 32 * TH), lds(at + 48 * TH)};
+    f4(x, i);
   }
-  float a, b;
-  unpack2(s2, a, b);
-  Part p;
-  p.m = m;
-  p.s = warp_sum(a + b);
-  unpack2(t2, a, b);
-  p.t = ENT ? warp_sum(a + b) : 0.0f;
-  p.w = -INFINITY;
-  return p;
+  for (; i < cnt; i += TH, at += 16 * TH) {
+    const uint4 x[1] = {lds(at)};
+    f1(x, i);
+  }
+}
+template <int TH, typename F> __device__ __forceinline__ void for_chunks(uint32_t st, int cnt, F &&f) {
+  for_chunks<TH>(st, cnt, [&](const uint4 (&x)[4], int i) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) f(x[k], i + k * TH);
+  }, [&](const uint4 (&x)[1], int i) { f(x[0], i); });
 }
 
-// The blocks of a row.  One block: barriers are the block's and no memory is
-// mapped.  A cluster: `arrive` then `wait` is a barrier of all its threads.
-template <bool CL> struct Team;
-template <> struct Team<false> {
-  static __device__ __forceinline__ unsigned rank() { return 0; }
-  static __device__ __forceinline__ unsigned size() { return 1; }
-  static __device__ __forceinline__ void arrive() {}
-  static __device__ __forceinline__ void wait() {}
-  static __device__ __forceinline__ void sync() { __syncthreads(); }
-  template <typename P> static __device__ __forceinline__ P *at(P *p, unsigned) { return p; }
+// This thread's running statistics of a row: m the largest logit so far, s and
+// t relative to it.
+struct Running {
+  float m = -FLT_MAX, top = -INFINITY;
+  f32x2 s2 = 0, t2 = 0;
+  template <typename T, bool ENT, int C> __device__ __forceinline__ void add(const uint4 (&x)[C], float c) {
+    constexpr int EV = Elem<T>::EV;
+    float b = Elem<T>::max_of(x[0]);
+#pragma unroll
+    for (int k = 1; k < C; k++) b = fmaxf(b, Elem<T>::max_of(x[k]));
+    top = fmaxf(top, b);
+    if (b > m) {                       // the sums move to the new reference
+      const float d = bounded((m - b) * c), f = exp2_fast(d);
+      const f32x2 f2 = pack2(f, f);
+      if (ENT) t2 = mul2(f2, fma2(s2, pack2(d, d), t2));
+      s2 = mul2(s2, f2);
+      m = b;
+    }
+    const f32x2 nm = pack2(-m, -m), cc = pack2(c, c);
+#pragma unroll
+    for (int k = 0; k < C; k++) {
+      float f[EV];
+      Elem<T>::unpack(x[k], f);
+#pragma unroll
+      for (int e = 0; e < EV; e += 2) {
+        float d0, d1;
+        unpack2(mul2(add2(pack2(f[e], f[e + 1]), nm), cc), d0, d1);
+        const f32x2 ex = pack2(exp2_fast(d0), exp2_fast(d1));
+        s2 = add2(s2, ex);
+        if (ENT) t2 = fma2(ex, pack2(bounded(d0), bounded(d1)), t2);
+      }
+    }
+  }
+  // The warp's part.
+  template <bool ENT> __device__ __forceinline__ Part warp(float c) const {
+    Part p = no_part();
+    p.m = warp_max(m);
+    const float d = bounded((m - p.m) * c), f = exp2_fast(d);
+    float a, b;
+    unpack2(s2, a, b);
+    const float s = a + b;
+    p.s = warp_sum(s * f);
+    if (ENT) {
+      unpack2(t2, a, b);
+      p.t = warp_sum(f * fmaf(s, d, a + b));
+    }
+    return p;
+  }
 };
-template <> struct Team<true> {
+template <typename T, int TH, bool ENT>
+__device__ __forceinline__ void add_share(Running &run, uint32_t st, int cnt, float c) {
+  for_chunks<TH>(st, cnt, [&](const uint4 (&x)[4], int) { run.add<T, ENT>(x, c); },
+                 [&](const uint4 (&x)[1], int) { run.add<T, ENT>(x, c); });
+}
+
+// The blocks of a row: `sync` is a barrier of all their threads.
+struct Team {
   static __device__ __forceinline__ unsigned rank() { return cg::this_cluster().block_rank(); }
   static __device__ __forceinline__ unsigned size() { return cg::this_cluster().num_blocks(); }
-  static __device__ __forceinline__ void arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
-  static __device__ __forceinline__ void wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-  static __device__ __forceinline__ void sync() { arrive(); wait(); }
+  static __device__ __forceinline__ void sync() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+  }
   template <typename P> static __device__ __forceinline__ P *at(P *p, unsigned r) {
     return cg::this_cluster().map_shared_rank(p, r);
   }
@@ -435,7 +470,7 @@ template <bool ENT> __device__ __forceinline__ Part join_all(const Part *part, i
 // and the next write of it.
 template <bool ENT>
 __device__ __forceinline__ void meet(const Part *part, Part *from, int g, float c) {
-  using TM = Team<true>;
+  using TM = Team;
   __syncthreads();
   if (threadIdx.x < 32) {
     Part p = join_all<ENT>(part, blockDim.x >> 5, c);
@@ -457,8 +492,8 @@ struct RowPlan {
 };
 RowPlan plan_rows(const DeviceCtx *c, const LogitRows &z, int K);
 // Launches a kernel over N rows: as many blocks (clusters of `blocks`) as the
-// GPU holds at once, each taking rows in turn.  `more_smem` bytes of dynamic
-// shared memory follow the stages, `args` is the kernel's one argument, `seen`
+// GPU holds at once, each taking rows in turn.  `more_threads` beside the
+// plan's in a block, `more_smem` bytes of dynamic shared memory after the stages, `args` is the kernel's one argument, `seen`
 // belongs to the kernel and the device: how many fit, for its latest shapes.
 struct Resident {
   static constexpr int N = 16;
@@ -468,6 +503,6 @@ struct Resident {
   int ready, next;
   Shape of[N];
 };
-int launch_rows(const void *kernel, DeviceCtx *c, const RowPlan &p, int more_smem, Resident *seen, void *args);
+int launch_rows(const void *kernel, DeviceCtx *c, const RowPlan &p, int more_threads, int more_smem, Resident *seen, void *args);
 
 }  // namespace tl

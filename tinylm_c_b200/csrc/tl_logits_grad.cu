@@ -115,224 +115,429 @@ struct DistillArgs {
 // + q_r (log q_r - log p_r), p_r = sum of p over the others; Q = sum q + q_r.
 //   named v:  dL/dy_v = Q p_v - q_v
 //   others:   dL/dy_v = p_v (Q - q_r / p_r)
-// The row is read once.  With a tail the named tokens are taken out of it (set
-// to -inf in shared memory) before its statistics, so that p_r is summed and
-// never 1 - sum p, which loses all its digits for a confident student.  All
-// others' gradients are then one factor times e_v; the named tokens' are
-// written over them at the end.
-template <typename T, bool CL, bool TAIL>
-__global__ void __launch_bounds__(MAX_THREADS, 2) distill_kernel(const DistillArgs a) {
-  using TM = Team<CL>;
-  constexpr int EV = Elem<T>::EV, KL = TL_TOPK_MAX / 32;
+// With a tail the named tokens are taken out of the row (set to -inf in shared
+// memory) before its statistics, so that p_r is summed and never 1 - sum p,
+// which loses all its digits for a confident student.  All others' gradients
+// are then one factor times e_v; the named tokens' are written over them at
+// the end.
+//
+// A row's entries in shared memory, K of each: the token (-1: padding), its q
+// and logit, and the mass of the token an entry stands for (-1 if it stands
+// for none: entries naming one token add up, the first of them stands for it).
+struct Entries {
+  int *id;
+  float *q, *z, *qv;
+  __device__ __forceinline__ Entries(void *p, int K, int flip)
+      : id(static_cast<int *>(p) + flip * 4 * K), q(static_cast<float *>(p) + (flip * 4 + 1) * K), z(q + K), qv(z + K) {}
+};
+constexpr int KL = TL_TOPK_MAX / 32;             // entries a lane
+
+// Row n's entries as one warp loads them.
+struct Loaded {
+  int id[KL];
+  float t[KL];
+  __device__ __forceinline__ void load(const DistillArgs &a, int n) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int k = 0; k < KL; k++) {
+      const int j = k * 32 + lane;
+      id[k] = -1;
+      t[k] = -INFINITY;
+      if (j < a.K) {
+        id[k] = a.t_ids[(size_t)n * a.K + j];
+        t[k] = a.t_vals[(size_t)n * a.K + j];
+      }
+    }
+  }
+};
+// The teacher's distribution from a row's loaded entries, by one warp: the
+// entries in shared memory, sum[0] the sum of q, sum[1] the tail.
+template <typename T, bool TAIL>
+__device__ __forceinline__ void teach(const DistillArgs &a, const Chunks<T> &r, Loaded &l, const Entries &to, float *sum) {
+  const int lane = threadIdx.x & 31;
+  float z[KL], tm = -FLT_MAX;
+#pragma unroll
+  for (int k = 0; k < KL; k++) {
+    if ((unsigned)l.id[k] >= (unsigned)a.l.V) {
+      if (l.id[k] != -1) atomicExch(a.err, ERR_TOKEN);
+      l.id[k] = -1;
+      l.t[k] = -INFINITY;
+    }
+    z[k] = l.id[k] >= 0 ? Elem<T>::to_f(r.row[l.id[k]]) : -INFINITY;
+    tm = fmaxf(tm, l.t[k]);
+  }
+  if (!TAIL) tm = warp_max(tm);
+  float q[KL], all = 0.0f;
+#pragma unroll
+  for (int k = 0; k < KL; k++) {
+    q[k] = l.id[k] < 0 ? 0.0f : expf(TAIL ? l.t[k] : (l.t[k] - tm) * a.inv_t);
+    all += q[k];
+  }
+  all = warp_sum(all);
+  const float inv = TAIL ? 1.0f : all == 0.0f ? 0.0f : 1.0f / all;
+#pragma unroll
+  for (int k = 0; k < KL; k++) {
+    const int j = k * 32 + lane;
+    if (j < a.K) {
+      to.id[j] = l.id[k];
+      to.q[j] = to.qv[j] = q[k] * inv;
+      to.z[j] = z[k];
+    }
+  }
+  if (lane == 0) {
+    float Q = TAIL || all == 0.0f ? all : 1.0f;
+    if (!(all < INFINITY)) Q = NAN;              // a NaN or +inf among the values
+    const float qr = TAIL ? 1.0f - Q : 0.0f;
+    sum[0] = Q;
+    sum[1] = qr < TAIL_MIN ? 0.0f : qr;          // NaN stays
+  }
+  __syncwarp();
+#pragma unroll
+  for (int k = 0; k < KL; k++) {
+    const int j = k * 32 + lane;
+    if (k * 32 < a.K) {
+      bool again = false;
+      for (int i = 0; i < a.K; i++) again |= to.id[i] == l.id[k] && i != j;
+      if (l.id[k] < 0) {
+        if (j < a.K) to.qv[j] = -1.0f;
+      } else if (again) {
+        float qv = 0.0f;
+        bool first = true;
+        for (int i = 0; i < a.K; i++)
+          if (to.id[i] == l.id[k]) {
+            qv += to.q[i];
+            first = first && i >= j;
+          }
+        to.qv[j] = first ? qv : -1.0f;
+      }
+    }
+  }
+}
+// The named tokens of a piece in shared memory set to -inf, by the warp that
+// loaded the entries.
+template <typename T> __device__ __forceinline__ void take_out(const Piece<T> &p, T *st, const Loaded &l) {
+  constexpr int EV = Elem<T>::EV;
+#pragma unroll
+  for (int k = 0; k < KL; k++) {
+    const int at = l.id[k] + p.r.mis - p.c0 * EV;              // element of the piece
+    if (l.id[k] >= 0 && at >= 0 && at < p.cnt * EV) st[at] = Elem<T>::none();
+  }
+  tc::fence_proxy_async();                       // a later copy into this stage comes after these writes
+}
+
+// What the gradient and the loss of a row go by, from its statistics p (with a
+// tail: of the tokens not named) and its entries; the same in every warp.
+struct RowLoss {
+  float m, all, f, total, qr;                    // e relative to p.m, times f, is relative to m; all: its sum
+  __device__ __forceinline__ RowLoss(const Part &p, const float *sum)
+      : m(p.m), all(p.s), f(1.0f), total(sum[0] + sum[1]), qr(sum[1]) {}
+  template <bool TAIL>
+  __device__ __forceinline__ void named(const DistillArgs &a, const Part &p, const Entries &s) {
+    if (!TAIL) return;
+    const int lane = threadIdx.x & 31;
+    for (int j = lane; j < a.K; j += 32) m = fmaxf(m, s.z[j]);
+    m = warp_max(m);
+    float sum = 0.0f;
+    for (int j = lane; j < a.K; j += 32)
+      if (!(s.qv[j] < 0.0f)) sum += exp2_fast((s.z[j] - m) * a.c);
+    f = exp2_fast(bounded((p.m - m) * a.c));
+    all = fmaf(p.s, f, warp_sum(sum));
+  }
+  template <bool TAIL>
+  __device__ __forceinline__ void write_loss(const DistillArgs &a, const Part &p, const Entries &s, int n, float w) const {
+    const int lane = threadIdx.x & 31;
+    const float ls = logf(all);
+    float L = 0.0f;
+    for (int j = lane; j < a.K; j += 32) {
+      const float qv = s.qv[j];
+      if (qv > 0.0f) L += qv * (logf(qv) - ((s.z[j] - m) * a.inv_t - ls));
+    }
+    L = warp_sum(L);
+    if (TAIL && qr > 0.0f) L += qr * (logf(qr) - (logf(p.s) + (p.m - m) * a.inv_t - ls));
+    if (all == 0.0f) L = total > 0.0f ? INFINITY : 0.0f;       // a student that allows no token
+    if (all != all || total != total) L = NAN;
+    L *= w;
+    if (lane == 0) {
+      if (a.loss) a.loss[n] = L;
+      if (a.loss64) a.loss64[n] = (double)L;
+    }
+  }
+  // The factor of e_v of the tokens not named; g = dL's factor.
+  template <bool TAIL> __device__ __forceinline__ float factor(const Part &p, float g) const {
+    return all == 0.0f ? 0.0f : g * (total * f / all - (TAIL && qr > 0.0f && p.s > 0.0f ? qr / p.s : 0.0f));
+  }
+};
+
+// A row's gradient rows: chunks of the row's own alignment go out 16 bytes at a
+// time where the gradient's rows have it too.
+template <typename T> struct Out {
+  static constexpr int EV = Elem<T>::EV;
+  Chunks<T> o;
+  const Chunks<T> &r;
+  bool same;
+  __device__ __forceinline__ Out(const DistillArgs &a, const Chunks<T> &r_, int n)
+      : o(static_cast<const T *>(a.dz) + (a.dz ? (size_t)n * a.ldd : 0), a.l.V), r(r_), same(o.mis == r_.mis) {}
+  __device__ __forceinline__ void each(int c, const float (&f)[EV]) const {
+    const int v = r.first(c);
+#pragma unroll
+    for (int e = 0; e < EV; e++)
+      if (v + e >= 0 && v + e < r.V) o.row[v + e] = Elem<T>::from_f(f[e]);
+  }
+  // The others' gradients of a piece in shared memory.
+  template <int TH>
+  __device__ __forceinline__ void piece(uint32_t st, int c0, int cnt, const Part &p, float c, float coef) const {
+    const int in0 = same ? max(0, r.full0 - c0) : cnt, in1 = same ? min(cnt, r.full1 - c0) : cnt;
+    uint4 *const out = o.base + c0;
+    const f32x2 nm2 = pack2(-p.m, -p.m), c2 = pack2(c, c), k2 = pack2(coef, coef);
+    for_chunks<TH>(st, cnt, [&](const uint4 &x, int i) {
+      float v[EV];
+      Elem<T>::unpack(x, v);
+#pragma unroll
+      for (int e = 0; e < EV; e += 2) {
+        float d0, d1;
+        unpack2(mul2(add2(pack2(v[e], v[e + 1]), nm2), c2), d0, d1);
+        unpack2(mul2(pack2(exp2_fast(d0), exp2_fast(d1)), k2), v[e], v[e + 1]);
+      }
+      if ((unsigned)(i - in0) < (unsigned)(in1 - in0)) out[i] = Elem<T>::pack(v);
+      else each(c0 + i, v);
+    });
+  }
+  __device__ __forceinline__ void zeros(int c0, int cnt, int t, int TH) const {
+    const float f[EV] = {};
+    for (int i = c0 + t; i < c0 + cnt; i += TH) {
+      if (same && i >= r.full0 && i < r.full1) o.base[i] = make_uint4(0, 0, 0, 0);
+      else each(i, f);
+    }
+  }
+  // The named tokens' gradients, those in chunks [c0, c0 + cnt).
+  __device__ __forceinline__ void named(const DistillArgs &a, const Entries &s, const RowLoss &l, float g, int c0, int cnt,
+                                        int t, int TH) const {
+    if (l.all == 0.0f) return;
+    for (int j = t; j < a.K; j += TH) {
+      const float q = s.qv[j];
+      if (q < 0.0f) continue;
+      const int id = s.id[j], at = (id + r.mis) / EV;
+      if (at < c0 || at >= c0 + cnt) continue;
+      const float p = exp2_fast((s.z[j] - l.m) * a.c) / l.all;
+      o.row[id] = Elem<T>::from_f(g * (l.total * p - q));
+    }
+  }
+};
+
+// Few rows, each split over the blocks of a cluster, a piece a block.
+template <typename T, int TH, bool TAIL>
+__global__ void __launch_bounds__(TH, min_blocks(TH)) distill_cluster_kernel(const DistillArgs a) {
+  using TM = Team;
+  constexpr int W = TH / 32;
   extern __shared__ __align__(128) unsigned char s_dyn[];
   // two of each, for rows in turn: a barrier of the next row lies between a
   // row's last reads and the row after that's writes
-  __shared__ Part s_part[2][MAX_WARPS], s_from[2][MAX_CLUSTER];
-  __shared__ float s_sum[2][2];                  // sum of q, the tail
-  __shared__ uint64_t s_full[MAX_STAGES];
+  __shared__ Part s_part[2][W], s_from[2][MAX_CLUSTER];
+  __shared__ float s_sum[2][2];
+  __shared__ uint64_t s_full;
   __shared__ int s_abort;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, TH = blockDim.x;
-  const int S = (int)TM::size();
-  const int rank = (int)TM::rank();
-  const Rows<T> t(a.l, rank);
-  const int N = a.l.N, V = a.l.V, stride = (int)gridDim.x / S, first_row = (int)blockIdx.x / S;
-  Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), a.l.stages, a.l.chunks, s_full, &s_abort, a.err};
-  // the row's entries: token (-1: padding), its q and logit, and the mass of
-  // the token an entry stands for (-1 if it stands for none)
-  float *s_entry = reinterpret_cast<float *>(s_dyn + (size_t)a.l.stages * a.l.chunks * 16);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int S = (int)TM::size(), rank = (int)TM::rank();
+  const Rows<T> t(a.l);
+  const int N = a.l.N, stride = (int)gridDim.x / S, first_row = (int)blockIdx.x / S;
+  const Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), 1, a.l.chunks, &s_full, &s_abort, a.err};
   auto counts = [&](int n) { return !a.weight || a.weight[n] != 0.0f; };
   if (tid == 0) {
-    pipe.init();
-    for (int i = 0; i < a.l.stages; i++)
-      if (first_row + i * stride < N) pipe.issue(t, first_row + i * stride, i, counts(first_row + i * stride));
+    tc::mbar_init(tc::smem_u32(&s_full), 1);
+    s_abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    pipe.issue(t, first_row, rank, 0, counts(first_row));
   }
   TM::sync();
-  for (int n = first_row, flip = 0; n < N; n += stride, flip ^= 1) {
-    const Share<T> sh(t, n);
-    const Chunks<T> &r = sh.r;
-    const Chunks<T> o(static_cast<const T *>(a.dz) + (a.dz ? (size_t)n * a.ldd : 0), V);
+  uint32_t phase = 0;
+  for (int n = first_row, flip = 0; n < N; n += stride, flip ^= 1, phase ^= 1) {
+    const Piece<T> pc(t, n, rank);
+    const Out<T> out(a, pc.r, n);
     const float w = a.weight ? a.weight[n] : 1.0f;
-    const int cnt = sh.cnt, ahead = n + a.l.stages * stride;
+    const int ahead = n + stride;
     const bool next_counts = tid == 0 && ahead < N && counts(ahead);
-    uint4 *st = pipe.stage();
-    int *s_id = reinterpret_cast<int *>(s_entry) + flip * 4 * a.K;
-    float *s_q = s_entry + flip * 4 * a.K + a.K, *s_z = s_q + a.K, *s_qv = s_z + a.K;
-    auto store = [&](int c, const float (&f)[EV]) {
-      if (o.mis == r.mis && c >= r.full0 && c < r.full1) {
-        o.base[c] = Elem<T>::pack(f);
-      } else {
-        const int v = r.first(c);
-#pragma unroll
-        for (int e = 0; e < EV; e++)
-          if (v + e >= 0 && v + e < V) o.row[v + e] = Elem<T>::from_f(f[e]);
-      }
-    };
+    const uint32_t st = tc::smem_u32(s_dyn);
+    const Entries s(s_dyn + (size_t)a.l.chunks * 16, a.K, flip);
     if (w == 0.0f) {                             // a row that does not count is not read
-      if (a.dz) {
-        const float f[EV] = {};
-        for (int i = tid; i < cnt; i += TH) store(sh.c0 + i, f);
-      }
+      if (a.dz) out.zeros(pc.c0, pc.cnt, tid, TH);
       if (rank == 0 && tid == 0) {
         if (a.loss) a.loss[n] = 0.0f;
         if (a.loss64) a.loss64[n] = 0.0;
       }
-      tc::mbar_wait(tc::smem_u32(&s_full[pipe.at]), pipe.phase, &s_abort, a.err, ERR_COPY);
+      pipe.wait(&s_full, phase);
       TM::sync();
-      if (tid == 0 && ahead < N) pipe.issue(t, ahead, pipe.at, next_counts);
-      pipe.next();
+      if (tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, next_counts);
       continue;
     }
-    // ---- the teacher's entries, by the first warp of every block
+    Loaded l;
     if (warp == 0) {
-      int id[KL];
-      float tv[KL], tm = -FLT_MAX;
-#pragma unroll
-      for (int k = 0; k < KL; k++) {
-        const int j = k * 32 + lane;
-        id[k] = -1;
-        tv[k] = -INFINITY;
-        if (j < a.K) {
-          id[k] = a.t_ids[(size_t)n * a.K + j];
-          tv[k] = a.t_vals[(size_t)n * a.K + j];
-        }
-      }
-      float zk[KL];
-#pragma unroll
-      for (int k = 0; k < KL; k++) {
-        if ((unsigned)id[k] >= (unsigned)V) {
-          if (id[k] != -1) atomicExch(a.err, ERR_TOKEN);
-          id[k] = -1;
-          tv[k] = -INFINITY;
-        }
-        zk[k] = id[k] >= 0 ? Elem<T>::to_f(r.row[id[k]]) : -INFINITY;
-        tm = fmaxf(tm, tv[k]);
-      }
-      if (!TAIL) tm = warp_max(tm);
-      float q[KL], sum = 0.0f;
-#pragma unroll
-      for (int k = 0; k < KL; k++) {
-        q[k] = id[k] < 0 ? 0.0f : expf(TAIL ? tv[k] : (tv[k] - tm) * a.inv_t);
-        sum += q[k];
-      }
-      sum = warp_sum(sum);
-      const float inv = TAIL ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-      for (int k = 0; k < KL; k++) {
-        const int j = k * 32 + lane;
-        if (j < a.K) {
-          s_id[j] = id[k];
-          s_q[j] = s_qv[j] = q[k] * inv;
-          s_z[j] = zk[k];
-        }
-      }
-      __syncwarp();
-      // entries naming one token add up; the first of them stands for it
-#pragma unroll
-      for (int k = 0; k < KL; k++) {
-        const int j = k * 32 + lane;
-        if (k * 32 < a.K) {
-          bool again = false;
-          for (int i = 0; i < a.K; i++) again |= s_id[i] == id[k] && i != j;
-          if (id[k] < 0) {
-            if (j < a.K) s_qv[j] = -1.0f;
-          } else if (again) {
-            float qv = 0.0f;
-            bool first = true;
-            for (int i = 0; i < a.K; i++)
-              if (s_id[i] == id[k]) {
-                qv += s_q[i];
-                first = first && i >= j;
-              }
-            s_qv[j] = first ? qv : -1.0f;
-          }
-        }
-      }
-      if (lane == 0) {
-        float Q = TAIL || sum == 0.0f ? sum : 1.0f;
-        if (!(sum < INFINITY)) Q = NAN;          // a NaN or +inf among the values
-        const float qr = TAIL ? 1.0f - Q : 0.0f;
-        s_sum[flip][0] = Q;
-        s_sum[flip][1] = qr < TAIL_MIN ? 0.0f : qr;            // NaN stays
-      }
-      if (TAIL) {
-        pipe.wait(t, sh);
-#pragma unroll
-        for (int k = 0; k < KL; k++) {
-          const int at = id[k] + r.mis - sh.c0 * EV;           // element of the share
-          if (id[k] >= 0 && at >= 0 && at < cnt * EV) reinterpret_cast<T *>(st)[at] = Elem<T>::none();
-        }
-        tc::fence_proxy_async();                 // a later copy into this stage comes after these writes
-      }
+      l.load(a, n);
+      teach<T, TAIL>(a, pc.r, l, s, s_sum[flip]);
     }
-    if (!TAIL || warp != 0) pipe.wait(t, sh);
-    if (TAIL) __syncthreads();
-    // ---- the row's statistics (with a tail: those of the tokens not named)
-    Part p = warp_part<T, false>(st, cnt, thread_max<T>(st, cnt), a.c);
-    if (lane == 0) s_part[flip][warp] = p;
-    if (CL) meet<false>(s_part[flip], s_from[flip], 0, a.c);
-    else __syncthreads();
-    p = join_all<false>(CL ? s_from[flip] : s_part[flip], CL ? S : TH >> 5, a.c);
-    const float Q = s_sum[flip][0], qr = s_sum[flip][1];
-    float m = p.m, all = p.s, f = 1.0f;          // e of the row is relative to p.m, times f to m
+    pipe.wait(&s_full, phase);
+    if (t.ragged) pc.mask_ends(pipe.stage(0), [&](int i) { return i % TH == tid; });
     if (TAIL) {
-      for (int j = lane; j < a.K; j += 32) m = fmaxf(m, s_z[j]);
-      m = warp_max(m);
-      float named = 0.0f;
-      for (int j = lane; j < a.K; j += 32)
-        if (!(s_qv[j] < 0.0f)) named += exp2_fast((s_z[j] - m) * a.c);
-      f = exp2_fast(bounded((p.m - m) * a.c));
-      all = fmaf(p.s, f, warp_sum(named));
+      if (warp == 0) take_out(pc, reinterpret_cast<T *>(s_dyn), l);
+      __syncthreads();
     }
-    const float total = Q + qr;
-    if (rank == 0 && warp == 0 && (a.loss || a.loss64)) {
-      const float ls = logf(all);
-      float L = 0.0f;
-      for (int j = lane; j < a.K; j += 32) {
-        const float qv = s_qv[j];
-        if (qv > 0.0f) L += qv * (logf(qv) - ((s_z[j] - m) * a.inv_t - ls));
-      }
-      L = warp_sum(L);
-      if (TAIL && qr > 0.0f) L += qr * (logf(qr) - (logf(p.s) + (p.m - m) * a.inv_t - ls));
-      if (all == 0.0f) L = total > 0.0f ? INFINITY : 0.0f;     // a student that allows no token
-      if (all != all || total != total) L = NAN;
-      L *= w;
-      if (lane == 0) {
-        if (a.loss) a.loss[n] = L;
-        if (a.loss64) a.loss64[n] = (double)L;
-      }
-    }
+    Running run;
+    add_share<T, TH, false>(run, st, pc.cnt, a.c);
+    Part p = run.warp<false>(a.c);
+    if (lane == 0) s_part[flip][warp] = p;
+    meet<false>(s_part[flip], s_from[flip], 0, a.c);
+    p = join_all<false>(s_from[flip], S, a.c);
+    RowLoss row(p, s_sum[flip]);
+    row.named<TAIL>(a, p, s);
+    if (rank == 0 && warp == 0 && (a.loss || a.loss64)) row.write_loss<TAIL>(a, p, s, n, w);
     const float g = w * a.scale * a.inv_t;
-    if (a.dz) {
-      const float coef =
-          all == 0.0f ? 0.0f : g * (total * f / all - (TAIL && qr > 0.0f && p.s > 0.0f ? qr / p.s : 0.0f));
-      const f32x2 nm2 = pack2(-p.m, -p.m), c2 = pack2(a.c, a.c), k2 = pack2(coef, coef);
-#pragma unroll 4
-      for (int i = tid; i < cnt; i += TH) {
-        float v[EV];
-        Elem<T>::unpack(st[i], v);
-#pragma unroll
-        for (int e = 0; e < EV; e += 2) {
-          float d0, d1;
-          unpack2(mul2(add2(pack2(v[e], v[e + 1]), nm2), c2), d0, d1);
-          unpack2(mul2(pack2(exp2_fast(d0), exp2_fast(d1)), k2), v[e], v[e + 1]);
-        }
-        store(sh.c0 + i, v);
+    if (a.dz) out.template piece<TH>(st, pc.c0, pc.cnt, p, a.c, row.factor<TAIL>(p, g));
+    __syncthreads();
+    if (tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, next_counts);
+    if (a.dz) out.named(a, s, row, g, pc.c0, pc.cnt, tid, TH);
+  }
+  TM::sync();                                    // no block leaves while another may write to it
+}
+
+// Rows of one block each, in pieces one after another: TH threads compute, one
+// more warp keeps the pieces coming and one reads the teacher's entries a row
+// ahead and takes the named tokens out of the pieces.  A row of one piece is
+// kept in shared memory between the statistics and the gradient, a longer one
+// comes a second time, from L2 if the rows in flight fit there.
+template <typename T, int TH, bool TAIL>
+__global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) distill_kernel(const DistillArgs a) {
+  constexpr int W = TH / 32;
+  extern __shared__ __align__(128) unsigned char s_dyn[];
+  __shared__ Part s_part[2][W];
+  __shared__ float s_sum[2][2], s_weight[2];
+  __shared__ uint64_t s_full[MAX_STAGES], s_ready[MAX_STAGES], s_free[MAX_STAGES], s_taught[2], s_spent[2];
+  __shared__ int s_abort;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Rows<T> t(a.l);
+  const int N = a.l.N, stride = (int)gridDim.x, first_row = (int)blockIdx.x, stages = a.l.stages, pieces = a.l.pieces;
+  const int passes = a.dz && pieces > 1 ? 2 : 1;
+  const bool made_ready = TAIL || t.ragged;
+  void *const entries = s_dyn + (size_t)stages * a.l.chunks * 16;
+  const Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), stages, a.l.chunks, s_full, &s_abort, a.err};
+  if (tid == 0) {
+    for (int i = 0; i < stages; i++) {
+      tc::mbar_init(tc::smem_u32(&s_full[i]), 1);
+      tc::mbar_init(tc::smem_u32(&s_ready[i]), 1);
+      tc::mbar_init(tc::smem_u32(&s_free[i]), W);
+    }
+    for (int i = 0; i < 2; i++) {
+      tc::mbar_init(tc::smem_u32(&s_taught[i]), 1);
+      tc::mbar_init(tc::smem_u32(&s_spent[i]), W);
+    }
+    s_abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  if (warp == W) {                               // ---- the pieces
+    Turn put;
+    int k = 0;
+    float w = a.weight ? a.weight[first_row] : 1.0f;
+    for (int n = first_row; n < N; n += stride) {
+      const bool read = w != 0.0f;
+      if (a.weight && n + stride < N) w = a.weight[n + stride];
+      for (int i = 0; read && i < passes * pieces; i++, k++) {
+        if (k >= stages) pipe.wait(&s_free[put.s], put.phase ^ 1);
+        if (lane == 0) pipe.issue(t, n, i % pieces, put.s, true);
+        __syncwarp();
+        put.next(stages);
       }
     }
-    __syncthreads();
-    if (tid == 0 && ahead < N) pipe.issue(t, ahead, pipe.at, next_counts);
-    pipe.next();
-    if (!a.dz || all == 0.0f) continue;
-    for (int j = tid; j < a.K; j += TH) {
-      const float q = s_qv[j];
-      if (q < 0.0f) continue;
-      const int id = s_id[j], at = (id + r.mis) / EV;
-      if (at < sh.c0 || at >= sh.c0 + cnt) continue;   // another block's
-      const float pv = exp2_fast((s_z[j] - m) * a.c) / all;
-      o.row[id] = Elem<T>::from_f(g * (total * pv - q));
-    }
+    return;
   }
-  if (CL) TM::sync();                            // no block leaves while another may write to it
+  if (warp == W + 1) {                           // ---- the teacher
+    Turn get;
+    Loaded next;
+    next.load(a, first_row);
+    float w_next = a.weight ? a.weight[first_row] : 1.0f;
+    int rows = 0;
+    for (int n = first_row; n < N; n += stride, rows++) {
+      const int flip = rows & 1;
+      Loaded l = next;
+      const float w = w_next;
+      if (n + stride < N) {
+        next.load(a, n + stride);
+        if (a.weight) w_next = a.weight[n + stride];
+      }
+      if (rows >= 2) pipe.wait(&s_spent[flip], ((rows >> 1) - 1) & 1);
+      if (w != 0.0f) teach<T, TAIL>(a, t.row(n), l, Entries(entries, a.K, flip), s_sum[flip]);
+      __syncwarp();
+      if (lane == 0) {
+        s_weight[flip] = w;
+        tc::mbar_arrive(tc::smem_u32(&s_taught[flip]));
+      }
+      for (int i = 0; made_ready && w != 0.0f && i < passes * pieces; i++) {
+        pipe.wait(&s_full[get.s], get.phase);
+        if (i < pieces) {                          // the second time the named tokens are written over anyway
+          const Piece<T> pc(t, n, i);
+          if (TAIL) take_out(pc, reinterpret_cast<T *>(pipe.stage(get.s)), l);
+          if (t.ragged) pc.mask_ends(pipe.stage(get.s), [&](int) { return lane == 0; });
+        }
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_ready[get.s]));
+        get.next(stages);
+      }
+    }
+    return;
+  }
+  // ---- the computing warps
+  Turn turn;
+  auto arrived = [&] {
+    pipe.wait(&s_full[turn.s], turn.phase);
+    if (made_ready) pipe.wait(&s_ready[turn.s], turn.phase);
+  };
+  auto done = [&] {
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_free[turn.s]));
+    turn.next(stages);
+  };
+  int rows = 0;
+  for (int n = first_row; n < N; n += stride, rows++) {
+    const int flip = rows & 1;
+    const Entries s(entries, a.K, flip);
+    const Chunks<T> r = t.row(n);
+    const Out<T> out(a, r, n);
+    pipe.wait(&s_taught[flip], (rows >> 1) & 1);
+    const float w = s_weight[flip];
+    if (w == 0.0f) {                             // a row that does not count is not read
+      if (a.dz) out.zeros(0, r.n, tid, TH);
+      if (tid == 0) {
+        if (a.loss) a.loss[n] = 0.0f;
+        if (a.loss64) a.loss64[n] = 0.0;
+      }
+    } else {
+      Running run;
+      for (int i = 0; i < pieces; i++) {
+        arrived();
+        add_share<T, TH, false>(run, tc::smem_u32(pipe.stage(turn.s)), max(0, min(r.n - i * t.per, t.per)), a.c);
+        if (pieces > 1 || !a.dz) done();
+      }
+      Part p = run.warp<false>(a.c);
+      if (lane == 0) s_part[flip][warp] = p;
+      bar_sync<TH>();
+      p = join_all<false>(s_part[flip], W, a.c);
+      RowLoss row(p, s_sum[flip]);
+      row.named<TAIL>(a, p, s);
+      const float g = w * a.scale * a.inv_t;
+      if (a.dz) {
+        const float coef = row.factor<TAIL>(p, g);
+        for (int i = 0; i < pieces; i++) {
+          if (pieces > 1) arrived();
+          out.template piece<TH>(tc::smem_u32(pipe.stage(turn.s)), i * t.per, max(0, min(r.n - i * t.per, t.per)), p, a.c,
+                                 coef);
+          done();
+        }
+        bar_sync<TH>();
+        out.named(a, s, row, g, 0, r.n, tid, TH);
+      }
+      if (warp == W - 1 && (a.loss || a.loss64)) row.write_loss<TAIL>(a, p, s, n, w);
+    }
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_spent[flip]));
+  }
 }
 
 }  // namespace lg
@@ -358,13 +563,21 @@ template <typename T> int grad_typed(DeviceCtx *c, const lg::GradArgs &a) {
   return launch_grad<T, 256>(c, nch, a);
 }
 
-template <typename T, bool CL, bool TAIL> int launch_distill(DeviceCtx *c, const RowPlan &pl, lg::DistillArgs a) {
+template <typename T, int TH, bool TAIL> int launch_cluster(DeviceCtx *c, const RowPlan &pl, lg::DistillArgs a) {
   static Resident seen[kMaxDevices];
-  return launch_rows((const void *)lg::distill_kernel<T, CL, TAIL>, c, pl, 32 * a.K, &seen[c->device], &a);
+  return launch_rows((const void *)lg::distill_cluster_kernel<T, TH, TAIL>, c, pl, 0, 32 * a.K, &seen[c->device], &a);
 }
-template <typename T> int distill_typed(DeviceCtx *c, const RowPlan &pl, const lg::DistillArgs &a, bool tail) {
-  if (pl.blocks > 1) return tail ? launch_distill<T, true, true>(c, pl, a) : launch_distill<T, true, false>(c, pl, a);
-  return tail ? launch_distill<T, false, true>(c, pl, a) : launch_distill<T, false, false>(c, pl, a);
+template <typename T, int TH, bool TAIL> int launch_distill(DeviceCtx *c, const RowPlan &pl, lg::DistillArgs a) {
+  static Resident seen[kMaxDevices];
+  return launch_rows((const void *)lg::distill_kernel<T, TH, TAIL>, c, pl, 64, 32 * a.K, &seen[c->device], &a);
+}
+template <typename T, bool TAIL> int distill_typed(DeviceCtx *c, const RowPlan &pl, const lg::DistillArgs &a) {
+  if (pl.blocks > 1) {
+    if (pl.threads == 128) return launch_cluster<T, 128, TAIL>(c, pl, a);
+    return pl.threads == 256 ? launch_cluster<T, 256, TAIL>(c, pl, a) : launch_cluster<T, 512, TAIL>(c, pl, a);
+  }
+  if (pl.threads == 32) return launch_distill<T, 32, TAIL>(c, pl, a);
+  return pl.threads == 128 ? launch_distill<T, 128, TAIL>(c, pl, a) : launch_distill<T, 256, TAIL>(c, pl, a);
 }
 
 }  // namespace
@@ -387,9 +600,10 @@ int k_distill_topk(DeviceCtx *c, const LogitRows &z, const int *t_ids, const flo
   const RowPlan pl = plan_rows(c, z, 0);
   const lg::DistillArgs a{pl.l, t_ids, t_vals, K, lg::LOG2E / temperature, 1.0f / temperature, weight, scale, loss,
                           loss64, dlogits, ldd, c->err_flag};
-  if (z.dtype == TL_F32) return distill_typed<float>(c, pl, a, tail);
-  if (z.dtype == TL_BF16) return distill_typed<__nv_bfloat16>(c, pl, a, tail);
-  return distill_typed<__half>(c, pl, a, tail);
+  if (z.dtype == TL_F32) return tail ? distill_typed<float, true>(c, pl, a) : distill_typed<float, false>(c, pl, a);
+  if (z.dtype == TL_BF16)
+    return tail ? distill_typed<__nv_bfloat16, true>(c, pl, a) : distill_typed<__nv_bfloat16, false>(c, pl, a);
+  return tail ? distill_typed<__half, true>(c, pl, a) : distill_typed<__half, false>(c, pl, a);
 }
 
 }  // namespace tl

@@ -41,10 +41,10 @@ __device__ __forceinline__ float value_of(unsigned long long key) {
 // at least K logits are at or above thr, or thr = -inf.  `first` is the share's
 // first element.  Every thread of the row's blocks calls it.  2 to 50 counting
 // passes over shared memory, of about a microsecond each.
-template <typename T, bool CL>
+template <typename T>
 __device__ __noinline__ void select_exactly(const uint4 *st, int cnt, int first, int V, int K, float thr,
                                             unsigned *s_count, unsigned long long *s_keys) {
-  using TM = Team<CL>;
+  using TM = Team;
   constexpr int EV = Elem<T>::EV;
   __shared__ int s_cnt[2][MAX_WARPS], s_sum[2][MAX_CLUSTER];
   const int tid = threadIdx.x, TH = blockDim.x, W = TH >> 5;
@@ -69,12 +69,10 @@ __device__ __noinline__ void select_exactly(const uint4 *st, int cnt, int first,
     __syncthreads();
     int sum = 0;
     for (int i = 0; i < W; i++) sum += s_cnt[flip][i];
-    if constexpr (CL) {
-      if (tid < (int)S) *TM::at(&s_sum[flip][TM::rank()], tid) = sum;
-      TM::sync();
-      sum = 0;
-      for (int i = 0; i < (int)S; i++) sum += s_sum[flip][i];
-    }
+    if (tid < (int)S) *TM::at(&s_sum[flip][TM::rank()], tid) = sum;
+    TM::sync();
+    sum = 0;
+    for (int i = 0; i < (int)S; i++) sum += s_sum[flip][i];
     flip ^= 1;
     return sum;
   };
@@ -115,26 +113,26 @@ __device__ __noinline__ void select_exactly(const uint4 *st, int cnt, int first,
   TM::sync();
 }
 
-// Keys in descending order, four a lane (lane l holds places 4l .. 4l + 3): a
-// bitonic sort of 128 in one warp.
-__device__ __forceinline__ void sort_128(unsigned long long (&k)[4]) {
+// Keys of a warp in descending order, R a lane (lane l holds places R l ...):
+// a bitonic sort of 32 R.
+template <int R> __device__ __forceinline__ void sort_keys(unsigned long long (&k)[R]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int size = 2; size <= 128; size <<= 1)
+  for (int size = 2; size <= 32 * R; size <<= 1)
 #pragma unroll
     for (int o = size >> 1; o; o >>= 1)
-      if (o >= 4) {
-        const bool larger = ((lane * 4 & o) == 0) == ((lane * 4 & size) == 0);
+      if (o >= R) {
+        const bool larger = ((lane * R & o) == 0) == ((lane * R & size) == 0);
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const unsigned long long u = __shfl_xor_sync(FULL, k[r], o >> 2);
+        for (int r = 0; r < R; r++) {
+          const unsigned long long u = __shfl_xor_sync(FULL, k[r], o / R);
           k[r] = (u > k[r]) == larger ? u : k[r];
         }
       } else {
 #pragma unroll
-        for (int r = 0; r < 4; r++)
+        for (int r = 0; r < R; r++)
           if (!(r & o)) {
-            const bool down = ((lane * 4 + r) & size) == 0;
+            const bool down = ((lane * R + r) & size) == 0;
             const unsigned long long x = k[r], y = k[r | o];
             const bool swap = (y > x) == down;
             k[r] = swap ? y : x;
@@ -154,35 +152,38 @@ struct ScoreArgs {
   int *err;
 };
 
-template <typename T, bool CL, bool ENT>
-__global__ void __launch_bounds__(MAX_THREADS, 2) score_kernel(const ScoreArgs a) {
-  using TM = Team<CL>;
-  constexpr int EV = Elem<T>::EV;
+// Few rows, each split over the blocks of a cluster, a piece a block.
+template <typename T, int TH, bool ENT>
+__global__ void __launch_bounds__(TH, min_blocks(TH)) score_cluster_kernel(const ScoreArgs a) {
+  using TM = Team;
+  constexpr int EV = Elem<T>::EV, W = TH / 32;
   extern __shared__ __align__(128) unsigned char s_dyn[];
-  __shared__ Part s_part[2][MAX_WARPS], s_from[2][MAX_CLUSTER];
+  __shared__ Part s_part[2][W], s_from[2][MAX_CLUSTER];
   __shared__ unsigned s_count[2];
-  __shared__ uint64_t s_full[MAX_STAGES];
+  __shared__ uint64_t s_full;
   __shared__ int s_abort;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, TH = blockDim.x, W = TH >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int S = (int)TM::size(), rank = (int)TM::rank();
-  const Rows<T> t(a.l, rank);
+  const Rows<T> t(a.l);
   const int N = a.l.N, stride = (int)gridDim.x / S, first_row = (int)blockIdx.x / S;
-  unsigned long long *s_keys = reinterpret_cast<unsigned long long *>(s_dyn + (size_t)a.l.stages * a.l.chunks * 16);
-  Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), a.l.stages, a.l.chunks, s_full, &s_abort, a.err};
+  unsigned long long *s_keys = reinterpret_cast<unsigned long long *>(s_dyn + (size_t)a.l.chunks * 16);
+  const Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), 1, a.l.chunks, &s_full, &s_abort, a.err};
   // full warps of this block, in every row: those whose 32 lanes all hold logits
-  const int mine = max(0, min(min((a.l.V + EV - 1) / EV - t.c0, t.per), TH)) >> 5;
+  const int mine = max(0, min(min((a.l.V + EV - 1) / EV - rank * t.per, t.per), TH)) >> 5;
   const int g = a.j ? (a.K * mine + a.j * a.g_full - 1) / (a.j * a.g_full) : 0;
   const bool reports = rank == 0 && tid == 0;    // the thread that writes a row's scalars
   if (tid == 0) {
-    pipe.init();
-    for (int i = 0; i < a.l.stages; i++)
-      if (first_row + i * stride < N) pipe.issue(t, first_row + i * stride, i, true);
+    tc::mbar_init(tc::smem_u32(&s_full), 1);
+    s_abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    pipe.issue(t, first_row, rank, 0, true);
     s_count[0] = s_count[1] = 0;
   }
   int id_next = reports && a.logp ? a.ids[first_row] : -1;
   TM::sync();
-  for (int n = first_row, flip = 0; n < N; n += stride, flip ^= 1) {
-    const Share<T> sh(t, n);
+  uint32_t phase = 0;
+  for (int n = first_row, flip = 0; n < N; n += stride, flip ^= 1, phase ^= 1) {
+    const Piece<T> sh(t, n, rank);
     // the given token's logit, and the next row's token
     int id = id_next;
     float z_id = 0.0f;
@@ -196,37 +197,33 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) score_kernel(const ScoreArgs a
       if (n + stride < N) id_next = a.ids[n + stride];
     }
     const int cnt = sh.cnt;
-    const uint4 *st = pipe.stage();
-    pipe.wait(t, sh);
-    const float top = thread_max<T>(st, cnt);
+    const uint32_t st = tc::smem_u32(s_dyn);
+    pipe.wait(&s_full, phase);
+    if (t.ragged) sh.mask_ends(pipe.stage(0), [&](int i) { return i % TH == tid; });
+    Running run;
+    add_share<T, TH, ENT>(run, st, cnt, a.c);
+    const float top = run.top;
     float w = -INFINITY;
     if (a.j && warp < mine) w = a.j == 1 ? warp_max(top) : nth_largest<32>(top, a.j);
-    Part p = warp_part<T, ENT>(st, cnt, top, a.c);
+    Part p = run.warp<ENT>(a.c);
     p.w = w;
     if (lane == 0) s_part[flip][warp] = p;
-    if (CL) meet<ENT>(s_part[flip], s_from[flip], g, a.c);
-    else __syncthreads();
-    const Part *parts = CL ? s_from[flip] : s_part[flip];
-    const int ahead = n + a.l.stages * stride;
-    if (!a.K && tid == 0 && ahead < N) pipe.issue(t, ahead, pipe.at, true);
+    meet<ENT>(s_part[flip], s_from[flip], g, a.c);
+    const Part *parts = s_from[flip];
+    const int ahead = n + stride;
+    if (!a.K && tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, true);
     unsigned found = 0;
     if (a.K) {                       // ---- the alternatives
       float thr = -INFINITY;         // too few maxima: every element passes
-      if (CL) {
-        if (a.j) {
-          thr = (lane & 15) < S ? parts[lane & 15].w : INFINITY;
+      if (a.j) {
+        thr = (lane & 15) < S ? parts[lane & 15].w : INFINITY;
 #pragma unroll
-          for (int o = 8; o; o >>= 1) thr = fminf(thr, __shfl_xor_sync(FULL, thr, o));
-        }
-      } else if (a.j) {
-        thr = W == 1 ? parts[0].w : nth_largest<16>((lane & 15) < W ? parts[lane & 15].w : -INFINITY, g);
+        for (int o = 8; o; o >>= 1) thr = fminf(thr, __shfl_xor_sync(FULL, thr, o));
       }
       unsigned *count = TM::at(&s_count[flip], 0);
       unsigned long long *keys = TM::at(s_keys, 0);
       if (top >= thr && top > -INFINITY) {
-#pragma unroll 2
-        for (int i = tid; i < cnt; i += TH) {
-          const uint4 x = st[i];
+        for_chunks<TH>(st, cnt, [&](const uint4 &x, int i) {
           if (Elem<T>::max_of(x) >= thr) {
             float f[EV];
             Elem<T>::unpack(x, f);
@@ -238,24 +235,24 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) score_kernel(const ScoreArgs a
                 if (at < CAP) keys[at] = key_of(f[e], v + e);
               }
           }
-        }
+        });
       }
       TM::sync();
       found = *count;
       if (found > CAP) {
-        const Part all = join_all<false>(parts, CL ? S : W, a.c);
+        const Part all = join_all<false>(parts, S, a.c);
         if (all.s >= 0.0f) {         // a row without a distribution has no alternatives
-          select_exactly<T, CL>(st, cnt, sh.r.first(sh.c0), t.V, a.K, thr, &s_count[flip], s_keys);
+          select_exactly<T>(pipe.stage(0), cnt, sh.r.first(sh.c0), t.V, a.K, thr, &s_count[flip], s_keys);
           found = *count;
         }
       }
-      if (tid == 0 && ahead < N) pipe.issue(t, ahead, pipe.at, true);
+      if (tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, true);
     }
     // ---- results: the first block's first warp, and all its warps where many
     // candidates are left to put in order
     const bool crowd = found > 128;
     if (rank == 0 && (warp == 0 || crowd)) {
-      p = join_all<ENT>(parts, CL ? S : W, a.c);
+      p = join_all<ENT>(parts, S, a.c);
       const float ls = logf(p.s);    // -inf where nothing is left, NaN for a row without a distribution
       const bool bad = !(p.s >= 0.0f);
       if (tid == 0) {
@@ -290,7 +287,7 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) score_kernel(const ScoreArgs a
           unsigned long long k[4];
 #pragma unroll
           for (int r = 0; r < 4; r++) k[r] = lane * 4 + r < got ? s_keys[lane * 4 + r] : 0;
-          sort_128(k);
+          sort_keys<4>(k);
 #pragma unroll
           for (int r = 0; r < 4; r++)
             if (lane * 4 + r < got) put(lane * 4 + r, k[r]);
@@ -302,26 +299,382 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) score_kernel(const ScoreArgs a
           }
       }
     }
-    pipe.next();
   }
-  if (CL) TM::sync();                // the first block's memory stays until all have read it
+  TM::sync();                // the first block's memory stays until all have read it
+}
+
+
+// ---- rows of one block each, in pieces one after another
+//
+// TH threads compute; one more warp keeps the pieces coming and one writes the
+// results, sorts the alternatives and looks the given tokens up, so that the
+// next row is under way meanwhile.  The warps hand over through barriers in
+// shared memory (a stage full, a stage free, a row's results there, taken).
+//
+// Alternatives over several pieces: the threshold is taken from the maxima of
+// the row so far after pieces 1, 2, 4, 8, ... and the last, and every element
+// above the threshold at hand is kept; where a piece's own maxima have moved
+// it, elements equal to it count as well (before that they cannot be among the
+// K: the K elements at or above it come earlier).
+constexpr int CROWD = 256;           // candidates that the results' warp puts in order
+
+// The K largest keys of a row in memory, where more than CAP elements passed:
+// at least K are at or above thr, or thr = -inf.  By TH threads (barrier 1):
+// bisection for the K-th largest value, counting over the row, then equal
+// logits in order of their index.
+template <typename T, int TH>
+__device__ __noinline__ void select_row(const T *row, int V, int K, float thr, uint2 *keys, unsigned *s_count) {
+  constexpr int EV = Elem<T>::EV, W = TH / 32;
+  __shared__ int s_cnt[2][W];
+  const Chunks<T> r(row, V);
+  const int tid = threadIdx.x, lane = tid & 31;
+  int flip = 0;
+  auto chunk = [&](int c, float (&f)[EV]) {
+    Elem<T>::unpack(c >= r.full0 && c < r.full1 ? __ldcg(r.base + c) : r.load_edge(c), f);
+  };
+  auto total = [&](int k) {
+    if (lane == 0) s_cnt[flip][tid >> 5] = k;
+    bar_sync<TH>();
+    int sum = 0;
+    for (int i = 0; i < W; i++) sum += s_cnt[flip][i];
+    flip ^= 1;
+    return sum;
+  };
+  auto at_least = [&](unsigned u) {                // elements of order u or above
+    int k = 0;
+#pragma unroll 1
+    for (int c = tid; c < r.n; c += TH) {
+      float f[EV];
+      chunk(c, f);
+#pragma unroll
+      for (int e = 0; e < EV; e++) k += f[e] > -INFINITY && order_of(f[e]) >= u;
+    }
+    return total(__reduce_add_sync(FULL, k));
+  };
+  // invariant: at least K of order lo or above; `above` < K of order hi or above.
+  // The first probe is the order just above the threshold: a mask of a type's
+  // lowest value leaves fewer than K above it.
+  unsigned lo = order_of(thr == -INFINITY ? -FLT_MAX : thr), hi = order_of(INFINITY), probe = lo + 1;
+  int above = 0;
+  bar_sync<TH>();                    // every thread has read s_count
+  while (hi - lo > 1) {
+    const int k = at_least(probe);
+    if (k >= K) {
+      lo = probe;
+    } else {
+      hi = probe;
+      above = k;
+    }
+    probe = lo + (hi - lo) / 2;
+  }
+  if (tid == 0) *s_count = 0;
+  bar_sync<TH>();
+#pragma unroll 1
+  for (int c = tid; above && c < r.n; c += TH) {
+    float f[EV];
+    chunk(c, f);
+#pragma unroll
+    for (int e = 0; e < EV; e++)
+      if (f[e] > -INFINITY && order_of(f[e]) > lo)
+        keys[atomicAdd(s_count, 1u)] = make_uint2(__float_as_uint(f[e]), (unsigned)(r.first(c) + e));
+  }
+  for (int c0 = 0, have = above; have < K && c0 < r.n; c0 += TH) {
+    float f[EV];
+    int k = 0;
+    if (c0 + tid < r.n) {
+      chunk(c0 + tid, f);
+#pragma unroll
+      for (int e = 0; e < EV; e++) k += f[e] > -INFINITY && order_of(f[e]) == lo;
+    }
+    int before = k;                  // of the warp's lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(FULL, before, o);
+      if (lane >= o) before += u;
+    }
+    const int warp_k = __shfl_sync(FULL, before, 31), mark = flip;
+    const int sum = total(warp_k);
+    int at = have + before - k;
+    for (int i = 0; i < tid >> 5; i++) at += s_cnt[mark][i];
+    if (k) {
+#pragma unroll
+      for (int e = 0; e < EV; e++)
+        if (f[e] > -INFINITY && order_of(f[e]) == lo && at < K)
+          keys[at++] = make_uint2(__float_as_uint(f[e]), (unsigned)(r.first(c0 + tid) + e));
+    }
+    have += sum;
+  }
+  bar_sync<TH>();
+  if (tid == 0) *s_count = K;
+  bar_sync<TH>();
+}
+
+template <typename T, int TH, bool ENT, bool TOP>
+__global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(const ScoreArgs a) {
+  constexpr int EV = Elem<T>::EV, W = TH / 32;
+  extern __shared__ __align__(128) unsigned char s_dyn[];
+  // two of each, for rows in turn
+  __shared__ Part s_part[2][W];
+  __shared__ float s_thr[2], s_w[2][W];
+  __shared__ unsigned s_count[2];
+  __shared__ uint64_t s_full[MAX_STAGES], s_ready[MAX_STAGES], s_free[MAX_STAGES], s_done[2], s_taken[2];
+  __shared__ int s_abort;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Rows<T> t(a.l);
+  const int N = a.l.N, stride = (int)gridDim.x, first_row = (int)blockIdx.x, stages = a.l.stages, pieces = a.l.pieces;
+  const Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), stages, a.l.chunks, s_full, &s_abort, a.err};
+  uint2 *s_keys = reinterpret_cast<uint2 *>(s_dyn + (size_t)stages * a.l.chunks * 16);     // [2][CAP]
+  if (tid == 0) {
+    for (int i = 0; i < stages; i++) {
+      tc::mbar_init(tc::smem_u32(&s_full[i]), 1);
+      tc::mbar_init(tc::smem_u32(&s_ready[i]), 1);
+      tc::mbar_init(tc::smem_u32(&s_free[i]), W);
+    }
+    for (int i = 0; i < 2; i++) {
+      tc::mbar_init(tc::smem_u32(&s_done[i]), W);
+      tc::mbar_init(tc::smem_u32(&s_taken[i]), 1);
+      s_count[i] = 0;
+    }
+    s_abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  if (warp == W) {                   // ---- the pieces
+    Turn put, get;
+    int gn = first_row, gi = 0, k = 0;             // the piece to be made ready
+    auto make_ready = [&] {
+      pipe.wait(&s_full[get.s], get.phase);
+      Piece<T>(t, gn, gi).mask_ends(pipe.stage(get.s), [&](int) { return lane == 0; });
+      if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_ready[get.s]));
+      get.next(stages);
+      if (++gi == pieces) { gi = 0; gn += stride; }
+    };
+    for (int n = first_row; n < N; n += stride)
+      for (int i = 0; i < pieces; i++, k++) {
+        if (k >= stages) pipe.wait(&s_free[put.s], put.phase ^ 1);
+        if (lane == 0) pipe.issue(t, n, i, put.s, true);
+        __syncwarp();
+        put.next(stages);
+        if (t.ragged && k >= stages - 1) make_ready();
+      }
+    if (t.ragged)
+      while (gn < N) make_ready();
+    return;
+  }
+  if (warp == W + 1) {               // ---- the results
+    int id = a.logp && lane == 0 ? a.ids[first_row] : -1;
+    uint32_t phase = 0;
+    for (int n = first_row, flip = 0; n < N; n += stride) {
+      float z_id = 0.0f;
+      const int given = id;
+      if (lane == 0 && a.logp) {
+        if (id >= 0 && id < t.V) z_id = Elem<T>::to_f(t.z[(size_t)n * t.ld + id]);
+        else if (id != -1) atomicExch(a.err, ERR_TOKEN);
+        if (n + stride < N) id = a.ids[n + stride];
+      }
+      pipe.wait(&s_done[flip], phase);
+      const Part p = join_all<ENT>(s_part[flip], W, a.c);
+      const float ls = logf(p.s);    // -inf where nothing is left, NaN for a row without a distribution
+      const bool bad = !(p.s >= 0.0f);
+      if (lane == 0) {
+        if (a.logp)
+          a.logp[n] = given < 0 || given >= t.V ? 0.0f : p.s == 0.0f ? -INFINITY : (z_id - p.m) * a.inv_t - ls;
+        if (ENT) {
+          const float h = ls - p.t / p.s * LN2;
+          a.entropy[n] = p.s == 0.0f || h < 0.0f ? 0.0f : h;
+        }
+        if (a.stats) {
+          a.stats[2 * (size_t)n] = p.m;
+          a.stats[2 * (size_t)n + 1] = p.s == 0.0f ? INFINITY : ls;
+        }
+      }
+      if (TOP) {
+        const int found = (int)s_count[flip];
+        const float thr = s_thr[flip];
+        const uint2 *keys = s_keys + flip * CAP;
+        int *to_id = a.top_ids + (size_t)n * a.K;
+        float *to_lp = a.top_logp + (size_t)n * a.K;
+        auto put = [&](int place, unsigned long long k) {
+          if (place >= a.K || !k) return;
+          to_id[place] = (int)(0xFFFFFFFFu - (unsigned)k);
+          to_lp[place] = (value_of(k) - p.m) * a.inv_t - ls;
+        };
+        auto key = [&](int i) -> unsigned long long {          // 0: none, or below the last threshold
+          if (i >= found) return 0;
+          const uint2 e = keys[i];
+          const float f = __uint_as_float(e.x);
+          return f >= thr ? key_of(f, (int)e.y) : 0;
+        };
+        int got = bad ? 0 : found > CROWD ? a.K : found;       // found > CROWD: already in its places
+        if (!bad && found <= 32) {
+          const unsigned long long k = key(lane);
+          int place = 0;
+          for (int q = 0; q < found; q++) place += __shfl_sync(FULL, k, q) > k;
+          put(place, k);
+          got = __popc(__ballot_sync(FULL, k != 0));
+        } else if (!bad && found <= CROWD) {
+          unsigned long long k[4], more = 0;
+#pragma unroll
+          for (int r = 0; r < 4; r++) k[r] = key(lane + 32 * r);
+          int below = 0;
+#pragma unroll
+          for (int r = 0; r < 4; r++) below += __popc(__ballot_sync(FULL, k[r] != 0));
+          for (int i = 128 + lane; i < (found + 31) / 32 * 32; i += 32) {
+            more = key(i);
+            below += __popc(__ballot_sync(FULL, more != 0));
+          }
+          got = below;
+          if (found <= 128) {
+            sort_keys<4>(k);
+#pragma unroll
+            for (int r = 0; r < 4; r++) put(lane * 4 + r, k[r]);
+          } else {
+            unsigned long long k8[8];
+#pragma unroll
+            for (int r = 0; r < 8; r++) k8[r] = key(lane + 32 * r);
+            sort_keys<8>(k8);
+#pragma unroll
+            for (int r = 0; r < 8; r++) put(lane * 8 + r, k8[r]);
+          }
+        }
+        for (int i = got + lane; i < a.K; i += 32) {
+          to_id[i] = -1;
+          to_lp[i] = bad ? NAN : -INFINITY;
+        }
+        __syncwarp();
+        if (lane == 0) s_count[flip] = 0;
+      }
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_taken[flip]));
+      flip ^= 1;
+      if (!flip) phase ^= 1;
+    }
+    return;
+  }
+  // ---- the computing warps
+  Turn turn;
+  int count_rows = 0, w_flip = 0;
+  for (int n = first_row; n < N; n += stride, count_rows++) {
+    const int flip = count_rows & 1;
+    // this row's places in shared memory: the results' warp has taken the row before last from them
+    if (count_rows >= 2) pipe.wait(&s_taken[flip], ((count_rows >> 1) - 1) & 1);
+    const Chunks<T> r = t.row(n);
+    uint2 *keys = s_keys + flip * CAP;
+    Running run;
+    float thr = TOP && a.j ? INFINITY : -INFINITY;
+    auto keep = [&](const uint4 &x, int c, bool equal) {       // chunk c's elements above the threshold
+      float f[EV];
+      Elem<T>::unpack(x, f);
+      const int v = r.first(c);
+#pragma unroll
+      for (int e = 0; e < EV; e++)
+        if ((f[e] > thr || (equal && f[e] == thr)) && f[e] > -INFINITY) {
+          const unsigned at = atomicAdd(&s_count[flip], 1u);
+          if (at < CAP) keys[at] = make_uint2(__float_as_uint(f[e]), (unsigned)(v + e));
+        }
+    };
+    for (int i = 0; i < pieces; i++) {
+      const int c0 = i * t.per, cnt = max(0, min(r.n - c0, t.per));
+      const uint32_t st = tc::smem_u32(pipe.stage(turn.s));
+      pipe.wait(&s_full[turn.s], turn.phase);
+      if (t.ragged) pipe.wait(&s_ready[turn.s], turn.phase);
+      if (!TOP) {
+        add_share<T, TH, ENT>(run, st, cnt, a.c);
+      } else if (a.j && ((i & (i + 1)) == 0 || i == pieces - 1)) {
+        add_share<T, TH, ENT>(run, st, cnt, a.c);
+        // warps whose lanes all have logits count (of the first piece: the
+        // others have no fewer, but the last)
+        const int mine = a.g_full;
+        float w = -INFINITY;
+        if (warp < mine) w = a.j == 1 ? warp_max(run.top) : nth_largest<32>(run.top, a.j);
+        if (W > 1) {
+          if (lane == 0) s_w[w_flip][warp] = w;
+          bar_sync<TH>();
+          w = (lane & 15) < W ? s_w[w_flip][lane & 15] : -INFINITY;
+          w = nth_largest<16>(w, (a.K + a.j - 1) / a.j);
+          w_flip ^= 1;
+        }
+        thr = w;
+        if (run.top >= thr)
+          for_chunks<TH>(st, cnt, [&](const uint4 &x, int k) {
+            if (Elem<T>::max_of(x) >= thr) keep(x, c0 + k, true);
+          });
+      } else {
+        for_chunks<TH>(st, cnt, [&](const uint4 (&x)[4], int k) {
+          run.add<T, ENT>(x, a.c);
+#pragma unroll
+          for (int q = 0; q < 4; q++)
+            if (Elem<T>::max_of(x[q]) > thr) keep(x[q], c0 + k + q * TH, false);
+        }, [&](const uint4 (&x)[1], int k) {
+          run.add<T, ENT>(x, a.c);
+          if (Elem<T>::max_of(x[0]) > thr) keep(x[0], c0 + k, false);
+        });
+      }
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_free[turn.s]));
+      turn.next(stages);
+    }
+    Part p = run.warp<ENT>(a.c);
+    if (lane == 0) s_part[flip][warp] = p;
+    if (TOP) {
+      if (tid == 0) s_thr[flip] = thr;
+      bar_sync<TH>();
+      const unsigned found = s_count[flip];
+      if (found > CROWD) {
+        p = join_all<false>(s_part[flip], W, a.c);
+        if (p.s >= 0.0f) {           // a row without a distribution has no alternatives
+          if (found > CAP) {
+            select_row<T, TH>(r.row, t.V, a.K, thr, keys, &s_count[flip]);
+          } else {
+            // so many that every thread finds its candidates' places
+            const float ls = logf(p.s);
+            for (int i = tid; i < (int)found; i += TH) {
+              const unsigned long long k = key_of(__uint_as_float(keys[i].x), (int)keys[i].y);
+              int place = 0;
+              for (int q = 0; q < (int)found; q++) place += key_of(__uint_as_float(keys[q].x), (int)keys[q].y) > k;
+              if (place < a.K) {
+                a.top_ids[(size_t)n * a.K + place] = (int)keys[i].y;
+                a.top_logp[(size_t)n * a.K + place] = (value_of(k) - p.m) * a.inv_t - ls;
+              }
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_done[flip]));
+  }
 }
 
 }  // namespace lg
 
 namespace {
 
-template <typename T, bool CL, bool ENT> int launch_score(DeviceCtx *c, const RowPlan &pl, lg::ScoreArgs a) {
+template <typename T, int TH, bool ENT> int launch_cluster(DeviceCtx *c, const RowPlan &pl, lg::ScoreArgs a) {
   static Resident seen[kMaxDevices];
-  return launch_rows((const void *)lg::score_kernel<T, CL, ENT>, c, pl, a.K ? lg::CAP * 8 : 0, &seen[c->device], &a);
+  return launch_rows((const void *)lg::score_cluster_kernel<T, TH, ENT>, c, pl, 0, a.K ? lg::CAP * 8 : 0,
+                     &seen[c->device], &a);
 }
-template <typename T> int score_typed(DeviceCtx *c, const RowPlan &pl, const lg::ScoreArgs &a) {
-  if (pl.blocks > 1) return a.entropy ? launch_score<T, true, true>(c, pl, a) : launch_score<T, true, false>(c, pl, a);
-  return a.entropy ? launch_score<T, false, true>(c, pl, a) : launch_score<T, false, false>(c, pl, a);
+template <typename T, int TH, bool ENT, bool TOP> int launch_score(DeviceCtx *c, const RowPlan &pl, lg::ScoreArgs a) {
+  static Resident seen[kMaxDevices];
+  return launch_rows((const void *)lg::score_kernel<T, TH, ENT, TOP>, c, pl, 64, TOP ? 2 * lg::CAP * 8 : 0,
+                     &seen[c->device], &a);
+}
+template <typename T, bool ENT, bool TOP> int score_rows(DeviceCtx *c, const RowPlan &pl, const lg::ScoreArgs &a) {
+  if (pl.threads == 32) return launch_score<T, 32, ENT, TOP>(c, pl, a);
+  return pl.threads == 128 ? launch_score<T, 128, ENT, TOP>(c, pl, a) : launch_score<T, 256, ENT, TOP>(c, pl, a);
+}
+template <typename T, bool ENT> int score_typed(DeviceCtx *c, const RowPlan &pl, const lg::ScoreArgs &a) {
+  if (pl.blocks > 1) {
+    if (pl.threads == 128) return launch_cluster<T, 128, ENT>(c, pl, a);
+    return pl.threads == 256 ? launch_cluster<T, 256, ENT>(c, pl, a) : launch_cluster<T, 512, ENT>(c, pl, a);
+  }
+  return a.K ? score_rows<T, ENT, true>(c, pl, a) : score_rows<T, ENT, false>(c, pl, a);
 }
 
-// What the threshold goes by: the row's full warps F (g_full) and the j of
-// "the j-th largest of a warp's 32 maxima", 0 where 32 F maxima are fewer than K.
+// What the threshold goes by: the full warps F (g_full) of the row, or of its
+// first piece, and the j of "the j-th largest of a warp's 32 maxima", 0 where
+// 32 F maxima are fewer than K.
 void threshold(const RowPlan &pl, int ev, lg::ScoreArgs *a) {
   const int nch = (a->l.V + ev - 1) / ev;        // chunks that every row has, whatever its alignment
   int full = 0;
@@ -330,8 +683,8 @@ void threshold(const RowPlan &pl, int ev, lg::ScoreArgs *a) {
   a->g_full = full;
   a->j = 0;
   if (!a->K || !full) return;
-  a->j = (5 * a->K + 4 * full - 1) / (4 * full);
-  if (a->j > 32) a->j = (a->K + full - 1) / full;
+  a->j = (a->K + full - 1) / full;
+  if (a->j < 4) a->j = (5 * a->K + 4 * full - 1) / (4 * full);
   if (a->j > 32) a->j = 0;
 }
 
@@ -344,9 +697,10 @@ int k_token_logprobs(DeviceCtx *c, const LogitRows &z, const int *ids, float tem
   lg::ScoreArgs a{pl.l, ids, lg::LOG2E / temperature, 1.0f / temperature, logp, entropy, stats, K, 0, 0, top_ids,
                   top_logp, c->err_flag};
   threshold(pl, z.dtype == TL_F32 ? 4 : 8, &a);
-  if (z.dtype == TL_F32) return score_typed<float>(c, pl, a);
-  if (z.dtype == TL_BF16) return score_typed<__nv_bfloat16>(c, pl, a);
-  return score_typed<__half>(c, pl, a);
+  if (z.dtype == TL_F32) return entropy ? score_typed<float, true>(c, pl, a) : score_typed<float, false>(c, pl, a);
+  if (z.dtype == TL_BF16)
+    return entropy ? score_typed<__nv_bfloat16, true>(c, pl, a) : score_typed<__nv_bfloat16, false>(c, pl, a);
+  return entropy ? score_typed<__half, true>(c, pl, a) : score_typed<__half, false>(c, pl, a);
 }
 
 }  // namespace tl
