@@ -40,7 +40,7 @@ RowPlan plan_rows(const DeviceCtx *c, const LogitRows &z, int K) {
 }
 
 int launch_rows(const void *kernel, DeviceCtx *c, const RowPlan &p, int more_threads, int more_smem, Resident *seen, void *args) {
-  constexpr int kMaxDynamic = 220 * 1024;          // of 227 KB a block may have, less the kernels' static part
+  constexpr int kMaxDynamic = 212 * 1024;          // of 227 KB a block may have, less the kernels' static part
   const int smem = p.l.stages * p.l.chunks * 16 + more_smem;
   if (smem > kMaxDynamic) return set_error(TL_EINVAL, "rows need %d bytes of shared memory a block", smem);
   cudaLaunchConfig_t cfg = {};

@@ -366,23 +366,27 @@ template <int N> __device__ __forceinline__ float nth_largest(float v, int j) {
   return __shfl_sync(FULL, v, j - 1);
 }
 
-// f(chunks, index of the first) for this thread's chunks tid, tid + TH, ... of
-// a share in shared memory, four at a time while four are left, then one.
-template <int TH, typename F4, typename F1>
+// f4(chunks, index of the first) for four of a thread's chunks tid, tid + TH,
+// ... of a piece in shared memory at a time while the whole warp has four left,
+// then f1 for one at a time; a lane without a chunk gets one of -inf.  The
+// warp's lanes stay together.
+template <typename T, int TH, typename F4, typename F1>
 __device__ __forceinline__ void for_chunks(uint32_t st, int cnt, F4 &&f4, F1 &&f1) {
-  int i = threadIdx.x;
+  const int lane = threadIdx.x & 31;
+  int i = threadIdx.x - lane;                      // of the warp's first lane
   uint32_t at = st + 16u * threadIdx.x;
-  for (; i + 3 * TH < cnt; i += 4 * TH, at += 64u * TH) {
+  for (; i + 3 * TH + 31 < cnt; i += 4 * TH, at += 64u * TH) {
     const uint4 x[4] = {lds(at), lds(at + 16 * TH), lds(at + 32 * TH), lds(at + 48 * TH)};
-    f4(x, i);
+    f4(x, i + lane);
   }
   for (; i < cnt; i += TH, at += 16 * TH) {
-    const uint4 x[1] = {lds(at)};
-    f1(x, i);
+    uint4 x[1] = {make_uint4(Elem<T>::FILL, Elem<T>::FILL, Elem<T>::FILL, Elem<T>::FILL)};
+    if (i + lane < cnt) x[0] = lds(at);
+    f1(x, i + lane);
   }
 }
-template <int TH, typename F> __device__ __forceinline__ void for_chunks(uint32_t st, int cnt, F &&f) {
-  for_chunks<TH>(st, cnt, [&](const uint4 (&x)[4], int i) {
+template <typename T, int TH, typename F> __device__ __forceinline__ void for_chunks(uint32_t st, int cnt, F &&f) {
+  for_chunks<T, TH>(st, cnt, [&](const uint4 (&x)[4], int i) {
 #pragma unroll
     for (int k = 0; k < 4; k++) f(x[k], i + k * TH);
   }, [&](const uint4 (&x)[1], int i) { f(x[0], i); });
@@ -439,7 +443,7 @@ struct Running {
 };
 template <typename T, int TH, bool ENT>
 __device__ __forceinline__ void add_share(Running &run, uint32_t st, int cnt, float c) {
-  for_chunks<TH>(st, cnt, [&](const uint4 (&x)[4], int) { run.add<T, ENT>(x, c); },
+  for_chunks<T, TH>(st, cnt, [&](const uint4 (&x)[4], int) { run.add<T, ENT>(x, c); },
                  [&](const uint4 (&x)[1], int) { run.add<T, ENT>(x, c); });
 }
 

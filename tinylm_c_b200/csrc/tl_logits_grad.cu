@@ -286,10 +286,10 @@ template <typename T> struct Out {
   // The others' gradients of a piece in shared memory.
   template <int TH>
   __device__ __forceinline__ void piece(uint32_t st, int c0, int cnt, const Part &p, float c, float coef) const {
-    const int in0 = same ? max(0, r.full0 - c0) : cnt, in1 = same ? min(cnt, r.full1 - c0) : cnt;
+    const int in0 = same ? max(0, r.full0 - c0) : cnt, in1 = same ? max(in0, min(cnt, r.full1 - c0)) : cnt;
     uint4 *const out = o.base + c0;
     const f32x2 nm2 = pack2(-p.m, -p.m), c2 = pack2(c, c), k2 = pack2(coef, coef);
-    for_chunks<TH>(st, cnt, [&](const uint4 &x, int i) {
+    for_chunks<T, TH>(st, cnt, [&](const uint4 &x, int i) {
       float v[EV];
       Elem<T>::unpack(x, v);
 #pragma unroll
@@ -299,7 +299,7 @@ template <typename T> struct Out {
         unpack2(mul2(pack2(exp2_fast(d0), exp2_fast(d1)), k2), v[e], v[e + 1]);
       }
       if ((unsigned)(i - in0) < (unsigned)(in1 - in0)) out[i] = Elem<T>::pack(v);
-      else each(c0 + i, v);
+      else if (i < cnt) each(c0 + i, v);
     });
   }
   __device__ __forceinline__ void zeros(int c0, int cnt, int t, int TH) const {

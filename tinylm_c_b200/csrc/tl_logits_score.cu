@@ -141,6 +141,41 @@ template <int R> __device__ __forceinline__ void sort_keys(unsigned long long (&
       }
 }
 
+// A warp's chunks whose largest logit passes, by their index in the piece, and
+// then their elements that pass, as many lanes a chunk as it has elements: few
+// chunks pass, and a warp that branched at each of them would run the elements'
+// code once for nearly every chunk (measured 1.6 times the whole kernel).
+struct Passing {
+  unsigned short *list;                          // 8 chunks a lane: 256
+  int n = 0;
+  __device__ __forceinline__ void add(bool pass, int i) {
+    const unsigned m = __ballot_sync(FULL, pass);
+    if (m) {
+      if (pass) list[n + __popc(m & ((1u << (threadIdx.x & 31)) - 1))] = (unsigned short)i;
+      n += __popc(m);
+    }
+  }
+  // push(element, its index in the piece) for the elements at or above (equal)
+  // or above thr.
+  template <typename T, typename F>
+  __device__ __forceinline__ void elements(const T *st, float thr, bool equal, F &&push) {
+    constexpr int EV = Elem<T>::EV;
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+    for (int b = 0; b < n; b += 32 / EV) {
+      const int q = b + lane / EV;
+      if (q < n) {
+        const int v = list[q] * EV + lane % EV;
+        const float f = Elem<T>::to_f(st[v]);
+        if ((f > thr || (equal && f == thr)) && f > -INFINITY) push(f, v);
+      }
+    }
+    __syncwarp();
+    n = 0;
+  }
+};
+constexpr int LIST = 256;                        // of a warp
+
 struct ScoreArgs {
   Layout l;
   const int *ids;
@@ -160,6 +195,7 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) score_cluster_kernel(const
   extern __shared__ __align__(128) unsigned char s_dyn[];
   __shared__ Part s_part[2][W], s_from[2][MAX_CLUSTER];
   __shared__ unsigned s_count[2];
+  __shared__ unsigned short s_list[W][LIST];
   __shared__ uint64_t s_full;
   __shared__ int s_abort;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -222,21 +258,19 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) score_cluster_kernel(const
       }
       unsigned *count = TM::at(&s_count[flip], 0);
       unsigned long long *keys = TM::at(s_keys, 0);
-      if (top >= thr && top > -INFINITY) {
-        for_chunks<TH>(st, cnt, [&](const uint4 &x, int i) {
-          if (Elem<T>::max_of(x) >= thr) {
-            float f[EV];
-            Elem<T>::unpack(x, f);
-            const int v = sh.r.first(sh.c0 + i);
-#pragma unroll
-            for (int e = 0; e < EV; e++)
-              if (f[e] >= thr && f[e] > -INFINITY) {
-                const unsigned at = atomicAdd(count, 1u);
-                if (at < CAP) keys[at] = key_of(f[e], v + e);
-              }
-          }
+      Passing pass{s_list[warp]};
+      auto flush = [&] {
+        pass.elements<T>(reinterpret_cast<const T *>(s_dyn), thr, true, [&](float f, int v) {
+          const unsigned at = atomicAdd(count, 1u);
+          if (at < CAP) keys[at] = key_of(f, sh.r.first(sh.c0) + v);
         });
-      }
+      };
+      for_chunks<T, TH>(st, cnt, [&](const uint4 &x, int i) {
+        const float m = Elem<T>::max_of(x);
+        pass.add(m >= thr && m > -INFINITY, i);
+        if (pass.n > LIST - 32) flush();
+      });
+      flush();
       TM::sync();
       found = *count;
       if (found > CAP) {
@@ -416,6 +450,7 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
   // two of each, for rows in turn
   __shared__ Part s_part[2][W];
   __shared__ float s_thr[2], s_w[2][W];
+  __shared__ unsigned short s_list[TOP ? W : 1][LIST];
   __shared__ unsigned s_count[2];
   __shared__ uint64_t s_full[MAX_STAGES], s_ready[MAX_STAGES], s_free[MAX_STAGES], s_done[2], s_taken[2];
   __shared__ int s_abort;
@@ -562,20 +597,11 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
     uint2 *keys = s_keys + flip * CAP;
     Running run;
     float thr = TOP && a.j ? INFINITY : -INFINITY;
-    auto keep = [&](const uint4 &x, int c, bool equal) {       // chunk c's elements above the threshold
-      float f[EV];
-      Elem<T>::unpack(x, f);
-      const int v = r.first(c);
-#pragma unroll
-      for (int e = 0; e < EV; e++)
-        if ((f[e] > thr || (equal && f[e] == thr)) && f[e] > -INFINITY) {
-          const unsigned at = atomicAdd(&s_count[flip], 1u);
-          if (at < CAP) keys[at] = make_uint2(__float_as_uint(f[e]), (unsigned)(v + e));
-        }
-    };
+    Passing pass{s_list[TOP ? warp : 0]};
     for (int i = 0; i < pieces; i++) {
       const int c0 = i * t.per, cnt = max(0, min(r.n - c0, t.per));
       const uint32_t st = tc::smem_u32(pipe.stage(turn.s));
+      bool equal = false;
       pipe.wait(&s_full[turn.s], turn.phase);
       if (t.ragged) pipe.wait(&s_ready[turn.s], turn.phase);
       if (!TOP) {
@@ -590,26 +616,30 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
         if (W > 1) {
           if (lane == 0) s_w[w_flip][warp] = w;
           bar_sync<TH>();
-          w = (lane & 15) < W ? s_w[w_flip][lane & 15] : -INFINITY;
-          w = nth_largest<16>(w, (a.K + a.j - 1) / a.j);
+          w = nth_largest<W>(s_w[w_flip][lane & (W - 1)], (a.K + a.j - 1) / a.j);
           w_flip ^= 1;
         }
         thr = w;
-        if (run.top >= thr)
-          for_chunks<TH>(st, cnt, [&](const uint4 &x, int k) {
-            if (Elem<T>::max_of(x) >= thr) keep(x, c0 + k, true);
-          });
+        equal = true;
+        for_chunks<T, TH>(st, cnt, [&](const uint4 &x, int k) {
+          const float m = Elem<T>::max_of(x);
+          pass.add(m >= thr && m > -INFINITY, k);
+        });
       } else {
-        for_chunks<TH>(st, cnt, [&](const uint4 (&x)[4], int k) {
+        for_chunks<T, TH>(st, cnt, [&](const uint4 (&x)[4], int k) {
           run.add<T, ENT>(x, a.c);
 #pragma unroll
-          for (int q = 0; q < 4; q++)
-            if (Elem<T>::max_of(x[q]) > thr) keep(x[q], c0 + k + q * TH, false);
+          for (int q = 0; q < 4; q++) pass.add(Elem<T>::max_of(x[q]) > thr, k + q * TH);
         }, [&](const uint4 (&x)[1], int k) {
           run.add<T, ENT>(x, a.c);
-          if (Elem<T>::max_of(x[0]) > thr) keep(x[0], c0 + k, false);
+          pass.add(Elem<T>::max_of(x[0]) > thr, k);
         });
       }
+      if (TOP)
+        pass.elements<T>(reinterpret_cast<const T *>(pipe.stage(turn.s)), thr, equal, [&](float f, int v) {
+          const unsigned at = atomicAdd(&s_count[flip], 1u);
+          if (at < CAP) keys[at] = make_uint2(__float_as_uint(f), (unsigned)(r.first(c0) + v));
+        });
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_free[turn.s]));
       turn.next(stages);
