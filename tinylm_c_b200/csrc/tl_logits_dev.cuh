@@ -397,7 +397,8 @@ template <typename T, int TH, typename F> __device__ __forceinline__ void for_ch
 struct Running {
   float m = -FLT_MAX, top = -INFINITY;
   f32x2 s2 = 0, t2 = 0;
-  template <typename T, bool ENT, int C> __device__ __forceinline__ void add(const uint4 (&x)[C], float c) {
+  // Adds C chunks; the largest of their logits.
+  template <typename T, bool ENT, int C> __device__ __forceinline__ float add(const uint4 (&x)[C], float c) {
     constexpr int EV = Elem<T>::EV;
     float b = Elem<T>::max_of(x[0]);
 #pragma unroll
@@ -424,6 +425,7 @@ struct Running {
         if (ENT) t2 = fma2(ex, pack2(bounded(d0), bounded(d1)), t2);
       }
     }
+    return b;
   }
   // The warp's part.
   template <bool ENT> __device__ __forceinline__ Part warp(float c) const {

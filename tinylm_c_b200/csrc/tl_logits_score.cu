@@ -2,17 +2,16 @@
 // entropy and its most likely tokens in one pass over the logits.
 //
 // The K most likely tokens.  A threshold below the K-th largest logit is found
-// without sorting the row.  Of the row's F full warps each takes the j-th
-// largest of its 32 lanes' maxima, j about 5/4 K / F; each block takes the
-// g-th largest of its F_b full warps' values, g = K F_b / (j F) rounded up;
-// the threshold is the least of the blocks'.  Every one of the g warps has j
-// elements at or above it, so the row has at least j sum g >= K.  Of random
-// logits 1.5 to 2 K pass (5/4: with j = 1 and all warps counted it is up to
-// 4.5 K, the least of many maxima being low).  They are collected in the first
-// block's shared memory as 64-bit keys (logit, then the lower index), and each
-// one's place is the number of larger keys.  Where more pass than the memory
-// holds (many equal logits, rows in order) the K-th largest key is found by
-// bisection, counting over the share, and exactly K are collected.
+// without sorting the row.  Of a block's F full warps each takes the j-th
+// largest of its 32 lanes' maxima; the threshold is the g-th largest of these,
+// g = K / j rounded up: every one of g warps has j elements at or above it.
+// j = K / F where that is 8 or more, else 5/4 of it, so that g < F: the least
+// of many maxima can be very low.  Of random logits 1.7 to 2.2 K pass.  (A
+// cluster's blocks take g in proportion to their full warps, and the least of
+// their thresholds.)  The elements that pass are collected in shared memory
+// and sorted as 64-bit keys: logit, then the lower index.  Where more pass than
+// the memory holds (many equal logits, rows in order) the K-th largest is
+// searched, counting over the row, and the lowest indices of equal ones taken.
 #include <algorithm>
 #include <cmath>
 #include "tl_logits_dev.cuh"
@@ -146,7 +145,7 @@ template <int R> __device__ __forceinline__ void sort_keys(unsigned long long (&
 // chunks pass, and a warp that branched at each of them would run the elements'
 // code once for nearly every chunk (measured 1.6 times the whole kernel).
 struct Passing {
-  unsigned short *list;                          // 8 chunks a lane: 256
+  unsigned short *list;                          // LIST of them
   int n = 0;
   __device__ __forceinline__ void add(bool pass, int i) {
     const unsigned m = __ballot_sync(FULL, pass);
@@ -174,14 +173,14 @@ struct Passing {
     n = 0;
   }
 };
-constexpr int LIST = 256;                        // of a warp
+constexpr int LIST = 160;                        // of a warp: four chunks a lane on top of a flush limit
 
 struct ScoreArgs {
   Layout l;
   const int *ids;
   float c, inv_t;                    // log2(e) / temperature, 1 / temperature
   float *logp, *entropy, *stats;
-  int K, j, g_full;                  // alternatives; see threshold() for j and g_full
+  int K, j, g_full, updates;         // alternatives; see threshold() for the others
   int *top_ids;
   float *top_logp;
   int *err;
@@ -346,100 +345,133 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) score_cluster_kernel(const
 // shared memory (a stage full, a stage free, a row's results there, taken).
 //
 // Alternatives over several pieces: the threshold is taken from the maxima of
-// the row so far after pieces 1, 2, 4, 8, ... and the last, and every element
-// above the threshold at hand is kept; where a piece's own maxima have moved
-// it, elements equal to it count as well (before that they cannot be among the
-// K: the K elements at or above it come earlier).
-constexpr int CROWD = 256;           // candidates that the results' warp puts in order
+// the row so far after piece 1, and after 2, 4, 8, ... until about 256 elements
+// of random logits pass in all.  Every element above the threshold at hand is
+// kept; in a piece whose own maxima have moved it, elements equal to it as well
+// (elsewhere they cannot be among the K: the K elements at or above it come
+// earlier).  A threshold of the whole row then leaves few to put in order.
 
-// The K largest keys of a row in memory, where more than CAP elements passed:
-// at least K are at or above thr, or thr = -inf.  By TH threads (barrier 1):
-// bisection for the K-th largest value, counting over the row, then equal
-// logits in order of their index.
+// The K largest keys of a row in memory (up to CAP with them), where more than
+// CAP elements passed: at least K are at or above thr, or thr = -inf.  By TH
+// threads (barrier 1), over the row in L2: one pass counts the elements at or
+// above the threshold and those above it.  Few enough are collected (the
+// row's last threshold is higher than those that filled the list); fewer than
+// K above it, as with a mask of a type's lowest value, leave equal logits to be
+// taken in order of their index; else the K-th largest value is searched, two
+// bits a pass.
 template <typename T, int TH>
 __device__ __noinline__ void select_row(const T *row, int V, int K, float thr, uint2 *keys, unsigned *s_count) {
   constexpr int EV = Elem<T>::EV, W = TH / 32;
-  __shared__ int s_cnt[2][W];
+  __shared__ int s_cnt[2][3][W];
   const Chunks<T> r(row, V);
   const int tid = threadIdx.x, lane = tid & 31;
   int flip = 0;
-  auto chunk = [&](int c, float (&f)[EV]) {
-    Elem<T>::unpack(c >= r.full0 && c < r.full1 ? __ldcg(r.base + c) : r.load_edge(c), f);
+  auto chunk = [&](int c) {
+    if (c >= r.full0 && c < r.full1) return __ldcg(r.base + c);
+    return c < r.n ? r.load_edge(c) : make_uint4(Elem<T>::FILL, Elem<T>::FILL, Elem<T>::FILL, Elem<T>::FILL);
   };
-  auto total = [&](int k) {
-    if (lane == 0) s_cnt[flip][tid >> 5] = k;
+  auto total = [&](const int (&k)[3], int (&sum)[3]) {
     bar_sync<TH>();
-    int sum = 0;
-    for (int i = 0; i < W; i++) sum += s_cnt[flip][i];
-    flip ^= 1;
-    return sum;
-  };
-  auto at_least = [&](unsigned u) {                // elements of order u or above
-    int k = 0;
-#pragma unroll 1
-    for (int c = tid; c < r.n; c += TH) {
-      float f[EV];
-      chunk(c, f);
 #pragma unroll
-      for (int e = 0; e < EV; e++) k += f[e] > -INFINITY && order_of(f[e]) >= u;
+    for (int q = 0; q < 3; q++) {
+      const int w = __reduce_add_sync(FULL, k[q]);
+      if (lane == 0) s_cnt[flip][q][tid >> 5] = w;
     }
-    return total(__reduce_add_sync(FULL, k));
+    bar_sync<TH>();
+#pragma unroll
+    for (int q = 0; q < 3; q++) {
+      sum[q] = 0;
+      for (int i = 0; i < W; i++) sum[q] += s_cnt[flip][q][i];
+    }
+    flip ^= 1;
   };
-  // invariant: at least K of order lo or above; `above` < K of order hi or above.
-  // The first probe is the order just above the threshold: a mask of a type's
-  // lowest value leaves fewer than K above it.
-  unsigned lo = order_of(thr == -INFINITY ? -FLT_MAX : thr), hi = order_of(INFINITY), probe = lo + 1;
-  int above = 0;
-  bar_sync<TH>();                    // every thread has read s_count
-  while (hi - lo > 1) {
-    const int k = at_least(probe);
-    if (k >= K) {
-      lo = probe;
-    } else {
-      hi = probe;
-      above = k;
+  // elements of order u[q] or above
+  auto at_least = [&](unsigned u0, unsigned u1, unsigned u2, int (&sum)[3]) {
+    int k[3] = {};
+#pragma unroll 1
+    for (int c = tid; c < r.n; c += 4 * TH) {
+      uint4 x[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[i] = chunk(c + i * TH);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        float f[EV];
+        Elem<T>::unpack(x[i], f);
+#pragma unroll
+        for (int e = 0; e < EV; e++) {
+          const unsigned o = f[e] > -INFINITY ? order_of(f[e]) : 0;
+          k[0] += o >= u0;
+          k[1] += o >= u1;
+          k[2] += o >= u2;
+        }
+      }
     }
-    probe = lo + (hi - lo) / 2;
+    total(k, sum);
+  };
+  // invariant: at least K of order lo or above; `above` < K of order hi or above
+  unsigned lo = order_of(thr == -INFINITY ? -FLT_MAX : thr), hi = order_of(INFINITY);
+  int sum[3], above = 0;
+  at_least(lo, lo + 1, hi, sum);
+  const bool few = sum[0] <= CAP;
+  if (few) {
+    hi = lo;                         // all of order lo or above are collected
+    above = sum[0];
+  } else if (sum[1] < K) {
+    hi = lo + 1;
+    above = sum[1];
+  }
+  while (!few && hi - lo > 1) {
+    const unsigned d = max((hi - lo) >> 2, 1u), u0 = lo + d, u1 = min(u0 + d, hi), u2 = min(u1 + d, hi);
+    at_least(u0, u1, u2, sum);
+    if (u2 < hi && sum[2] >= K) {
+      lo = u2;
+    } else {
+      if (u2 < hi) { hi = u2; above = sum[2]; }
+      if (u1 < hi && sum[1] >= K) {
+        lo = u1;
+      } else {
+        if (u1 < hi) { hi = u1; above = sum[1]; }
+        if (sum[0] >= K) lo = u0;
+        else { hi = u0; above = sum[0]; }
+      }
+    }
   }
   if (tid == 0) *s_count = 0;
   bar_sync<TH>();
 #pragma unroll 1
   for (int c = tid; above && c < r.n; c += TH) {
     float f[EV];
-    chunk(c, f);
+    Elem<T>::unpack(chunk(c), f);
 #pragma unroll
     for (int e = 0; e < EV; e++)
-      if (f[e] > -INFINITY && order_of(f[e]) > lo)
+      if (f[e] > -INFINITY && order_of(f[e]) >= hi)
         keys[atomicAdd(s_count, 1u)] = make_uint2(__float_as_uint(f[e]), (unsigned)(r.first(c) + e));
   }
-  for (int c0 = 0, have = above; have < K && c0 < r.n; c0 += TH) {
+  int have = above;
+  for (int c0 = 0; have < K && c0 < r.n; c0 += TH) {
     float f[EV];
+    Elem<T>::unpack(chunk(c0 + tid), f);
     int k = 0;
-    if (c0 + tid < r.n) {
-      chunk(c0 + tid, f);
 #pragma unroll
-      for (int e = 0; e < EV; e++) k += f[e] > -INFINITY && order_of(f[e]) == lo;
-    }
+    for (int e = 0; e < EV; e++) k += f[e] > -INFINITY && order_of(f[e]) == lo;
     int before = k;                  // of the warp's lanes up to this one
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(FULL, before, o);
       if (lane >= o) before += u;
     }
-    const int warp_k = __shfl_sync(FULL, before, 31), mark = flip;
-    const int sum = total(warp_k);
+    const int mark = flip, mine[3] = {k, 0, 0};
+    total(mine, sum);
     int at = have + before - k;
-    for (int i = 0; i < tid >> 5; i++) at += s_cnt[mark][i];
-    if (k) {
+    for (int i = 0; i < tid >> 5; i++) at += s_cnt[mark][0][i];
 #pragma unroll
-      for (int e = 0; e < EV; e++)
-        if (f[e] > -INFINITY && order_of(f[e]) == lo && at < K)
-          keys[at++] = make_uint2(__float_as_uint(f[e]), (unsigned)(r.first(c0 + tid) + e));
-    }
-    have += sum;
+    for (int e = 0; e < EV; e++)
+      if (f[e] > -INFINITY && order_of(f[e]) == lo && at < K)
+        keys[at++] = make_uint2(__float_as_uint(f[e]), (unsigned)(r.first(c0 + tid) + e));
+    have += sum[0];
   }
   bar_sync<TH>();
-  if (tid == 0) *s_count = K;
+  if (tid == 0) *s_count = few ? above : K;
   bar_sync<TH>();
 }
 
@@ -524,53 +556,55 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
         }
       }
       if (TOP) {
-        const int found = (int)s_count[flip];
+        const int found = bad ? 0 : (int)s_count[flip];
         const float thr = s_thr[flip];
-        const uint2 *keys = s_keys + flip * CAP;
+        uint2 *keys = s_keys + flip * CAP;
         int *to_id = a.top_ids + (size_t)n * a.K;
         float *to_lp = a.top_logp + (size_t)n * a.K;
+        int got = 0;                 // the candidates at or above the last threshold, to the front
+        for (int i = 0; i < found; i += 32) {
+          const uint2 e = i + lane < found ? keys[i + lane] : make_uint2(0xFF800000u, 0);
+          const unsigned m = __ballot_sync(FULL, __uint_as_float(e.x) >= thr && i + lane < found);
+          __syncwarp();
+          if (m >> lane & 1) keys[got + __popc(m & ((1u << lane) - 1))] = e;
+          got += __popc(m);
+        }
+        __syncwarp();
+        auto key = [&](int i) -> unsigned long long {
+          if (i >= got) return 0;
+          const uint2 e = keys[i];
+          return key_of(__uint_as_float(e.x), (int)e.y);
+        };
         auto put = [&](int place, unsigned long long k) {
           if (place >= a.K || !k) return;
           to_id[place] = (int)(0xFFFFFFFFu - (unsigned)k);
           to_lp[place] = (value_of(k) - p.m) * a.inv_t - ls;
         };
-        auto key = [&](int i) -> unsigned long long {          // 0: none, or below the last threshold
-          if (i >= found) return 0;
-          const uint2 e = keys[i];
-          const float f = __uint_as_float(e.x);
-          return f >= thr ? key_of(f, (int)e.y) : 0;
+        auto in_order = [&](auto &k) {
+          constexpr int R = sizeof(k) / sizeof(k[0]);
+#pragma unroll
+          for (int r = 0; r < R; r++) k[r] = key(lane + 32 * r);
+          sort_keys<R>(k);
+#pragma unroll
+          for (int r = 0; r < R; r++) put(lane * R + r, k[r]);
         };
-        int got = bad ? 0 : found > CROWD ? a.K : found;       // found > CROWD: already in its places
-        if (!bad && found <= 32) {
+        if (got <= 16) {
           const unsigned long long k = key(lane);
           int place = 0;
-          for (int q = 0; q < found; q++) place += __shfl_sync(FULL, k, q) > k;
+          for (int q = 0; q < got; q++) place += __shfl_sync(FULL, k, q) > k;
           put(place, k);
-          got = __popc(__ballot_sync(FULL, k != 0));
-        } else if (!bad && found <= CROWD) {
-          unsigned long long k[4], more = 0;
-#pragma unroll
-          for (int r = 0; r < 4; r++) k[r] = key(lane + 32 * r);
-          int below = 0;
-#pragma unroll
-          for (int r = 0; r < 4; r++) below += __popc(__ballot_sync(FULL, k[r] != 0));
-          for (int i = 128 + lane; i < (found + 31) / 32 * 32; i += 32) {
-            more = key(i);
-            below += __popc(__ballot_sync(FULL, more != 0));
-          }
-          got = below;
-          if (found <= 128) {
-            sort_keys<4>(k);
-#pragma unroll
-            for (int r = 0; r < 4; r++) put(lane * 4 + r, k[r]);
-          } else {
-            unsigned long long k8[8];
-#pragma unroll
-            for (int r = 0; r < 8; r++) k8[r] = key(lane + 32 * r);
-            sort_keys<8>(k8);
-#pragma unroll
-            for (int r = 0; r < 8; r++) put(lane * 8 + r, k8[r]);
-          }
+        } else if (got <= 32) {
+          unsigned long long k[1];
+          in_order(k);
+        } else if (got <= 128) {
+          unsigned long long k[4];
+          in_order(k);
+        } else if (got <= 256) {
+          unsigned long long k[8];
+          in_order(k);
+        } else {
+          unsigned long long k[16];
+          in_order(k);
         }
         for (int i = got + lane; i < a.K; i += 32) {
           to_id[i] = -1;
@@ -598,48 +632,66 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
     Running run;
     float thr = TOP && a.j ? INFINITY : -INFINITY;
     Passing pass{s_list[TOP ? warp : 0]};
+    // A value that at least K logits of the row so far are at or above, from
+    // the warps whose lanes all had logits in the first piece.
+    auto threshold = [&] {
+      float w = -INFINITY;
+      if (warp < a.g_full) w = a.j == 1 ? warp_max(run.top) : nth_largest<32>(run.top, a.j);
+      if (W > 1) {
+        if (lane == 0) s_w[w_flip][warp] = w;
+        bar_sync<TH>();
+        w = nth_largest<W>(s_w[w_flip][lane & (W - 1)], (a.K + a.j - 1) / a.j);
+        w_flip ^= 1;
+      }
+      return w;
+    };
     for (int i = 0; i < pieces; i++) {
       const int c0 = i * t.per, cnt = max(0, min(r.n - c0, t.per));
       const uint32_t st = tc::smem_u32(pipe.stage(turn.s));
       bool equal = false;
-      pipe.wait(&s_full[turn.s], turn.phase);
-      if (t.ragged) pipe.wait(&s_ready[turn.s], turn.phase);
-      if (!TOP) {
-        add_share<T, TH, ENT>(run, st, cnt, a.c);
-      } else if (a.j && ((i & (i + 1)) == 0 || i == pieces - 1)) {
-        add_share<T, TH, ENT>(run, st, cnt, a.c);
-        // warps whose lanes all have logits count (of the first piece: the
-        // others have no fewer, but the last)
-        const int mine = a.g_full;
-        float w = -INFINITY;
-        if (warp < mine) w = a.j == 1 ? warp_max(run.top) : nth_largest<32>(run.top, a.j);
-        if (W > 1) {
-          if (lane == 0) s_w[w_flip][warp] = w;
-          bar_sync<TH>();
-          w = nth_largest<W>(s_w[w_flip][lane & (W - 1)], (a.K + a.j - 1) / a.j);
-          w_flip ^= 1;
-        }
-        thr = w;
-        equal = true;
-        for_chunks<T, TH>(st, cnt, [&](const uint4 &x, int k) {
-          const float m = Elem<T>::max_of(x);
-          pass.add(m >= thr && m > -INFINITY, k);
-        });
-      } else {
-        for_chunks<T, TH>(st, cnt, [&](const uint4 (&x)[4], int k) {
-          run.add<T, ENT>(x, a.c);
-#pragma unroll
-          for (int q = 0; q < 4; q++) pass.add(Elem<T>::max_of(x[q]) > thr, k + q * TH);
-        }, [&](const uint4 (&x)[1], int k) {
-          run.add<T, ENT>(x, a.c);
-          pass.add(Elem<T>::max_of(x[0]) > thr, k);
-        });
-      }
-      if (TOP)
+      auto flush = [&] {
         pass.elements<T>(reinterpret_cast<const T *>(pipe.stage(turn.s)), thr, equal, [&](float f, int v) {
           const unsigned at = atomicAdd(&s_count[flip], 1u);
           if (at < CAP) keys[at] = make_uint2(__float_as_uint(f), (unsigned)(r.first(c0) + v));
         });
+      };
+      pipe.wait(&s_full[turn.s], turn.phase);
+      if (t.ragged) pipe.wait(&s_ready[turn.s], turn.phase);
+      if (!TOP) {
+        add_share<T, TH, ENT>(run, st, cnt, a.c);
+      } else if (a.j && (i & (i + 1)) == 0 && i + 1 < 2 * a.updates) {
+        add_share<T, TH, ENT>(run, st, cnt, a.c);
+        thr = threshold();
+        equal = true;
+        for_chunks<T, TH>(st, cnt, [&](const uint4 (&x)[4], int k) {
+          float m[4];
+#pragma unroll
+          for (int q = 0; q < 4; q++) m[q] = Elem<T>::max_of(x[q]);
+          const float b = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+          if (__any_sync(FULL, b >= thr && b > -INFINITY)) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) pass.add(m[q] >= thr && m[q] > -INFINITY, k + q * TH);
+            if (pass.n > LIST - 4 * 32) flush();
+          }
+        }, [&](const uint4 (&x)[1], int k) {
+          const float m = Elem<T>::max_of(x[0]);
+          pass.add(m >= thr && m > -INFINITY, k);
+          if (pass.n > LIST - 4 * 32) flush();
+        });
+      } else {
+        for_chunks<T, TH>(st, cnt, [&](const uint4 (&x)[4], int k) {
+          const float m = run.add<T, ENT>(x, a.c);
+          if (__any_sync(FULL, m > thr)) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) pass.add(Elem<T>::max_of(x[q]) > thr, k + q * TH);
+            if (pass.n > LIST - 4 * 32) flush();
+          }
+        }, [&](const uint4 (&x)[1], int k) {
+          pass.add(run.add<T, ENT>(x, a.c) > thr, k);
+          if (pass.n > LIST - 4 * 32) flush();
+        });
+      }
+      if (TOP) flush();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_free[turn.s]));
       turn.next(stages);
@@ -647,28 +699,13 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
     Part p = run.warp<ENT>(a.c);
     if (lane == 0) s_part[flip][warp] = p;
     if (TOP) {
+      if (a.j && pieces > 1) thr = fmaxf(thr, threshold());
       if (tid == 0) s_thr[flip] = thr;
       bar_sync<TH>();
-      const unsigned found = s_count[flip];
-      if (found > CROWD) {
+      if (s_count[flip] > CAP) {
         p = join_all<false>(s_part[flip], W, a.c);
-        if (p.s >= 0.0f) {           // a row without a distribution has no alternatives
-          if (found > CAP) {
-            select_row<T, TH>(r.row, t.V, a.K, thr, keys, &s_count[flip]);
-          } else {
-            // so many that every thread finds its candidates' places
-            const float ls = logf(p.s);
-            for (int i = tid; i < (int)found; i += TH) {
-              const unsigned long long k = key_of(__uint_as_float(keys[i].x), (int)keys[i].y);
-              int place = 0;
-              for (int q = 0; q < (int)found; q++) place += key_of(__uint_as_float(keys[q].x), (int)keys[q].y) > k;
-              if (place < a.K) {
-                a.top_ids[(size_t)n * a.K + place] = (int)keys[i].y;
-                a.top_logp[(size_t)n * a.K + place] = (value_of(k) - p.m) * a.inv_t - ls;
-              }
-            }
-          }
-        }
+        if (p.s >= 0.0f)             // a row without a distribution has no alternatives
+          select_row<T, TH>(r.row, t.V, a.K, thr, keys, &s_count[flip]);
       }
     }
     __syncwarp();
@@ -704,17 +741,21 @@ template <typename T, bool ENT> int score_typed(DeviceCtx *c, const RowPlan &pl,
 
 // What the threshold goes by: the full warps F (g_full) of the row, or of its
 // first piece, and the j of "the j-th largest of a warp's 32 maxima", 0 where
-// 32 F maxima are fewer than K.
+// 32 F maxima are fewer than K; `updates` pieces at most go by before the last
+// threshold that elements are kept by.
 void threshold(const RowPlan &pl, int ev, lg::ScoreArgs *a) {
   const int nch = (a->l.V + ev - 1) / ev;        // chunks that every row has, whatever its alignment
   int full = 0;
   for (int i = 0; i < pl.blocks; i++)
     full += std::max(0, std::min(std::min(nch - i * a->l.per, a->l.per), pl.threads)) / 32;
   a->g_full = full;
+  // of random logits 2 to 2.5 K of a threshold's part of the row pass, as many
+  // again of each further part of that length: kept below 256
+  a->updates = std::max(1, (a->K * a->l.pieces + 99) / 100);
   a->j = 0;
   if (!a->K || !full) return;
   a->j = (a->K + full - 1) / full;
-  if (a->j < 4) a->j = (5 * a->K + 4 * full - 1) / (4 * full);
+  if (a->j < 8) a->j = (5 * a->K + 4 * full - 1) / (4 * full);
   if (a->j > 32) a->j = 0;
 }
 
@@ -724,7 +765,7 @@ int k_token_logprobs(DeviceCtx *c, const LogitRows &z, const int *ids, float tem
                      float *entropy, float *stats, int K, int *top_ids, float *top_logp) {
   TraceScope ts(c, "k_token_logprobs");
   const RowPlan pl = plan_rows(c, z, K);
-  lg::ScoreArgs a{pl.l, ids, lg::LOG2E / temperature, 1.0f / temperature, logp, entropy, stats, K, 0, 0, top_ids,
+  lg::ScoreArgs a{pl.l, ids, lg::LOG2E / temperature, 1.0f / temperature, logp, entropy, stats, K, 0, 0, 0, top_ids,
                   top_logp, c->err_flag};
   threshold(pl, z.dtype == TL_F32 ? 4 : 8, &a);
   if (z.dtype == TL_F32) return entropy ? score_typed<float, true>(c, pl, a) : score_typed<float, false>(c, pl, a);
