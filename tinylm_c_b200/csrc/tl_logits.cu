@@ -13,7 +13,7 @@
 
 namespace tl {
 
-RowPlan plan_rows(const DeviceCtx *c, const LogitRows &z, int K) {
+RowPlan plan_rows(const DeviceCtx *c, const LogitRows &z, int K, bool twice) {
   const int es = z.dtype == TL_F32 ? 4 : 2, ev = 16 / es;
   // chunks of a row: its own alignment where all rows share it, else the worst
   const bool one = (z.ld * es) % 16 == 0 || z.N == 1;
@@ -29,11 +29,11 @@ RowPlan plan_rows(const DeviceCtx *c, const LogitRows &z, int K) {
     p.l.pieces = blocks;
     p.threads = p.l.per <= 512 ? 128 : p.l.per <= 2048 ? 256 : 512;
   } else {
-    p.threads = nch <= 256 && K <= 16 ? 32 : K > 64 ? 256 : 128;
-    const int per = K > 0 ? 2048 : 1024;
+    p.threads = nch <= 256 && K <= 16 ? 32 : nch <= 1024 ? 128 : twice || K > 64 ? 256 : 128;
+    const int per = twice || K > 0 ? 2048 : 1024;
     p.l.per = nch < per ? nch : per;
     p.l.pieces = (nch + p.l.per - 1) / p.l.per;
-    p.l.stages = p.threads == 32 ? 4 : K > 0 ? 1 : 2;
+    p.l.stages = p.threads == 32 ? 4 : !twice && K > 0 ? 1 : twice && p.l.pieces >= 6 ? 3 : 2;
   }
   p.l.chunks = (p.l.per + 7) / 8 * 8;
   p.l.ragged = !one || mis || (z.V % ev) != 0;

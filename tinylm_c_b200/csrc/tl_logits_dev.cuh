@@ -87,6 +87,24 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// What L2 should do with the lines of a copy: let them go first, keep them, or
+// nothing special.
+__device__ __forceinline__ uint64_t l2_once() {
+  uint64_t p;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ uint64_t l2_again() {
+  uint64_t p;
+  asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ uint64_t l2_normal() {
+  uint64_t p;
+  asm("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+
 // 16 bytes of shared memory at a 32-bit address.
 __device__ __forceinline__ uint4 lds(uint32_t a) {
   uint4 v;
@@ -279,7 +297,7 @@ template <typename T> struct Pipe {
   // at once), by one thread.  The stage's earlier readers are done.  The
   // tensor's first and last chunk, where it does not fill them, are written
   // by the calling thread.
-  __device__ __forceinline__ void issue(const Rows<T> &t, int n, int piece, int s, bool read) const {
+  __device__ __forceinline__ void issue(const Rows<T> &t, int n, int piece, int s, bool read, uint64_t policy) const {
     const uint32_t bar = tc::smem_u32(&full[s]);
     if (*(volatile int *)abort_flag) return;
     int lo = 0, hi = 0;
@@ -303,10 +321,11 @@ template <typename T> struct Pipe {
     const uint32_t bytes = (uint32_t)(hi - lo) * 16u;
     tc::mbar_arrive_expect_tx(bar, bytes);
     if (bytes)
-      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                       tc::smem_u32(st + lo)),
-                   "l"(__cvta_generic_to_global(from + lo)), "r"(bytes), "r"(bar)
-                   : "memory");
+      asm volatile(
+          "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
+              tc::smem_u32(st + lo)),
+          "l"(__cvta_generic_to_global(from + lo)), "r"(bytes), "r"(bar), "l"(policy)
+          : "memory");
   }
   // Waits for a phase of a barrier, for two seconds at most.  After an expired
   // wait the kernel runs on over what there is, its copies and waits over, and
@@ -496,7 +515,7 @@ struct RowPlan {
   int threads, blocks;
   lg::Layout l;
 };
-RowPlan plan_rows(const DeviceCtx *c, const LogitRows &z, int K);
+RowPlan plan_rows(const DeviceCtx *c, const LogitRows &z, int K, bool twice);
 // Launches a kernel over N rows: as many blocks (clusters of `blocks`) as the
 // GPU holds at once, each taking rows in turn.  `more_threads` beside the
 // plan's in a block, `more_smem` bytes of dynamic shared memory after the stages, `args` is the kernel's one argument, `seen`

@@ -284,7 +284,8 @@ template <typename T> struct Out {
       if (v + e >= 0 && v + e < r.V) o.row[v + e] = Elem<T>::from_f(f[e]);
   }
   // The others' gradients of a piece in shared memory.
-  template <int TH>
+  // ONCE: the row's other pieces are to stay in L2 meanwhile.
+  template <int TH, bool ONCE>
   __device__ __forceinline__ void piece(uint32_t st, int c0, int cnt, const Part &p, float c, float coef) const {
     const int in0 = same ? max(0, r.full0 - c0) : cnt, in1 = same ? max(in0, min(cnt, r.full1 - c0)) : cnt;
     uint4 *const out = o.base + c0;
@@ -298,8 +299,13 @@ template <typename T> struct Out {
         unpack2(mul2(add2(pack2(v[e], v[e + 1]), nm2), c2), d0, d1);
         unpack2(mul2(pack2(exp2_fast(d0), exp2_fast(d1)), k2), v[e], v[e + 1]);
       }
-      if ((unsigned)(i - in0) < (unsigned)(in1 - in0)) out[i] = Elem<T>::pack(v);
-      else if (i < cnt) each(c0 + i, v);
+      if ((unsigned)(i - in0) < (unsigned)(in1 - in0)) {
+        if (ONCE) __stcs(out + i, Elem<T>::pack(v));
+        else out[i] = Elem<T>::pack(v);
+      }
+      else if (i < cnt) {
+        each(c0 + i, v);
+      }
     });
   }
   __device__ __forceinline__ void zeros(int c0, int cnt, int t, int TH) const {
@@ -346,7 +352,7 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) distill_cluster_kernel(con
     tc::mbar_init(tc::smem_u32(&s_full), 1);
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    pipe.issue(t, first_row, rank, 0, counts(first_row));
+    pipe.issue(t, first_row, rank, 0, counts(first_row), l2_normal());
   }
   TM::sync();
   uint32_t phase = 0;
@@ -366,7 +372,7 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) distill_cluster_kernel(con
       }
       pipe.wait(&s_full, phase);
       TM::sync();
-      if (tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, next_counts);
+      if (tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, next_counts, l2_normal());
       continue;
     }
     Loaded l;
@@ -390,9 +396,9 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) distill_cluster_kernel(con
     row.named<TAIL>(a, p, s);
     if (rank == 0 && warp == 0 && (a.loss || a.loss64)) row.write_loss<TAIL>(a, p, s, n, w);
     const float g = w * a.scale * a.inv_t;
-    if (a.dz) out.template piece<TH>(st, pc.c0, pc.cnt, p, a.c, row.factor<TAIL>(p, g));
+    if (a.dz) out.template piece<TH, false>(st, pc.c0, pc.cnt, p, a.c, row.factor<TAIL>(p, g));
     __syncthreads();
-    if (tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, next_counts);
+    if (tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, next_counts, l2_normal());
     if (a.dz) out.named(a, s, row, g, pc.c0, pc.cnt, tid, TH);
   }
   TM::sync();                                    // no block leaves while another may write to it
@@ -434,6 +440,7 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) distill_kernel(c
   __syncthreads();
   if (warp == W) {                               // ---- the pieces
     Turn put;
+    const uint64_t first = passes == 2 ? l2_again() : l2_normal(), last = l2_once();
     int k = 0;
     float w = a.weight ? a.weight[first_row] : 1.0f;
     for (int n = first_row; n < N; n += stride) {
@@ -441,7 +448,7 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) distill_kernel(c
       if (a.weight && n + stride < N) w = a.weight[n + stride];
       for (int i = 0; read && i < passes * pieces; i++, k++) {
         if (k >= stages) pipe.wait(&s_free[put.s], put.phase ^ 1);
-        if (lane == 0) pipe.issue(t, n, i % pieces, put.s, true);
+        if (lane == 0) pipe.issue(t, n, i % pieces, put.s, true, i < pieces ? first : last);
         __syncwarp();
         put.next(stages);
       }
@@ -524,10 +531,14 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) distill_kernel(c
       const float g = w * a.scale * a.inv_t;
       if (a.dz) {
         const float coef = row.factor<TAIL>(p, g);
-        for (int i = 0; i < pieces; i++) {
-          if (pieces > 1) arrived();
-          out.template piece<TH>(tc::smem_u32(pipe.stage(turn.s)), i * t.per, max(0, min(r.n - i * t.per, t.per)), p, a.c,
-                                 coef);
+        if (pieces == 1) {
+          out.template piece<TH, false>(tc::smem_u32(pipe.stage(turn.s)), 0, r.n, p, a.c, coef);
+          done();
+        }
+        for (int i = 0; pieces > 1 && i < pieces; i++) {
+          arrived();
+          out.template piece<TH, true>(tc::smem_u32(pipe.stage(turn.s)), i * t.per, max(0, min(r.n - i * t.per, t.per)),
+                                       p, a.c, coef);
           done();
         }
         bar_sync<TH>();
@@ -597,7 +608,7 @@ int k_distill_topk(DeviceCtx *c, const LogitRows &z, const int *t_ids, const flo
                    float temperature, int tail, const float *weight, float scale, float *loss, double *loss64,
                    void *dlogits, long long ldd) {
   TraceScope ts(c, "k_distill_topk");
-  const RowPlan pl = plan_rows(c, z, 0);
+  const RowPlan pl = plan_rows(c, z, 0, true);
   const lg::DistillArgs a{pl.l, t_ids, t_vals, K, lg::LOG2E / temperature, 1.0f / temperature, weight, scale, loss,
                           loss64, dlogits, ldd, c->err_flag};
   if (z.dtype == TL_F32) return tail ? distill_typed<float, true>(c, pl, a) : distill_typed<float, false>(c, pl, a);

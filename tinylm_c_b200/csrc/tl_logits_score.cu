@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) score_cluster_kernel(const
     tc::mbar_init(tc::smem_u32(&s_full), 1);
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    pipe.issue(t, first_row, rank, 0, true);
+    pipe.issue(t, first_row, rank, 0, true, l2_once());
     s_count[0] = s_count[1] = 0;
   }
   int id_next = reports && a.logp ? a.ids[first_row] : -1;
@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) score_cluster_kernel(const
     meet<ENT>(s_part[flip], s_from[flip], g, a.c);
     const Part *parts = s_from[flip];
     const int ahead = n + stride;
-    if (!a.K && tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, true);
+    if (!a.K && tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, true, l2_once());
     unsigned found = 0;
     if (a.K) {                       // ---- the alternatives
       float thr = -INFINITY;         // too few maxima: every element passes
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) score_cluster_kernel(const
           found = *count;
         }
       }
-      if (tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, true);
+      if (tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, true, l2_once());
     }
     // ---- results: the first block's first warp, and all its warps where many
     // candidates are left to put in order
@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
     for (int n = first_row; n < N; n += stride)
       for (int i = 0; i < pieces; i++, k++) {
         if (k >= stages) pipe.wait(&s_free[put.s], put.phase ^ 1);
-        if (lane == 0) pipe.issue(t, n, i, put.s, true);
+        if (lane == 0) pipe.issue(t, n, i, put.s, true, l2_once());
         __syncwarp();
         put.next(stages);
         if (t.ragged && k >= stages - 1) make_ready();
@@ -764,7 +764,7 @@ void threshold(const RowPlan &pl, int ev, lg::ScoreArgs *a) {
 int k_token_logprobs(DeviceCtx *c, const LogitRows &z, const int *ids, float temperature, float *logp,
                      float *entropy, float *stats, int K, int *top_ids, float *top_logp) {
   TraceScope ts(c, "k_token_logprobs");
-  const RowPlan pl = plan_rows(c, z, K);
+  const RowPlan pl = plan_rows(c, z, K, false);
   lg::ScoreArgs a{pl.l, ids, lg::LOG2E / temperature, 1.0f / temperature, logp, entropy, stats, K, 0, 0, 0, top_ids,
                   top_logp, c->err_flag};
   threshold(pl, z.dtype == TL_F32 ? 4 : 8, &a);
