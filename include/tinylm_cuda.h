@@ -294,6 +294,26 @@ int tl_distill_topk(const void *logits, int dtype, long long ld, const int *t_id
                     int V, float temperature, int tail, const float *weight, float scale, float *loss, void *dlogits,
                     long long ldd);
 
+/* The device model's answers and its training on a teacher's, on the two
+ * operators above (fp32 logits, the model's vocabulary; arrays of B*T rows in
+ * the order of tok, B a multiple of the model's micro-batch).
+ * tl_model_score: log p of each target token, the entropy of each position's
+ * distribution and its K most likely tokens, as tl_token_logprobs gives them
+ * (tgt and logp together; each output may be NULL). */
+int tl_model_score(void *handle, const float *P, const int *tok, const int *tgt, int B, float temperature, float *logp,
+                   float *entropy, int K, int *top_ids, float *top_logp);
+/* tl_model_distill: loss = sum_n loss[n] / (B*T) with the rows' losses of
+ * tl_distill_topk (t_ids, t_vals [B*T][K], weight [B*T] or NULL), and
+ * G += its gradient (G NULL: the loss alone; loss_dev may be NULL if G is
+ * not).  A teacher says nothing of the MTP heads: they get no gradient. */
+int tl_model_distill(void *handle, const float *P, float *G, const int *tok, const int *t_ids, const float *t_vals,
+                     int K, const float *weight, int B, float temperature, int tail, float *loss_dev);
+/* memset(G) -> tl_model_distill -> norm -> clip(max_norm) -> AdamW(lr, 0.9,
+ * 0.95, 0.1, t), as tl_model_step does for the targets' loss. */
+int tl_model_distill_step(void *handle, float *P, float *G, float *M, float *V, const int *tok, const int *t_ids,
+                          const float *t_vals, int K, const float *weight, int B, float temperature, int tail, float lr,
+                          int t, float max_norm, float *loss_dev, float *norm_dev);
+
 /* ------------------------------------- training loop: host-side pieces */
 /* Checkpoints in the reference's formats.  Buffers may be host or device
  * memory (device data is staged through the host).

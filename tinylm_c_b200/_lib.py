@@ -93,6 +93,13 @@ SIGNATURES = {
                                        _c_int, _c_float, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
     "tl_distill_topk": (_c_int, [_c_void_p, _c_int, _c_longlong, _c_void_p, _c_void_p, _c_int, _c_int, _c_int,
                                  _c_float, _c_int, _c_void_p, _c_float, _c_void_p, _c_void_p, _c_longlong]),
+    "tl_model_score": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_float, _c_void_p, _c_void_p,
+                                _c_int, _c_void_p, _c_void_p]),
+    "tl_model_distill": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p,
+                                  _c_int, _c_float, _c_int, _c_void_p]),
+    "tl_model_distill_step": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                                       _c_void_p, _c_int, _c_void_p, _c_int, _c_float, _c_int, _c_float, _c_int,
+                                       _c_float, _c_void_p, _c_void_p]),
     "tl_zero1_padded": (_c_size, [_c_size, _c_int]),
     "tl_dist_unique_id": (_c_int, [_c_void_p]),
     "tl_dist_init": (_c_int, [_c_int, _c_int, _c_void_p]),

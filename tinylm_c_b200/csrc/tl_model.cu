@@ -16,6 +16,7 @@
 #include <cstring>
 #include <vector>
 #include "tl_gemm.cuh"
+#include "tl_logits.cuh"
 #include "tl_model.cuh"
 #include "tl_dist.cuh"
 #include "tl_trace.cuh"
@@ -108,15 +109,12 @@ static int gemm_add(DeviceCtx *c, GemmOp op, float *C, const float *A, const flo
   return gemm_run_add(c, op, C, A, B, M, K, N, add);
 }
 
-// One micro-batch: forward + backward, gradients accumulated into G.
-// ov (data-parallel step only, last micro-batch): told after each layer which
-// tail of G is final, so shard reductions start during the backward pass.
-static int micro_step(DeviceCtx *c, Model &m, const float *P, float *G, const int *tok, const int *tgt,
-                      const int *const *tgt_mtp, float scale, bool backward, OverlapState *ov = nullptr) {
+// One micro-batch's logits (tinylm.c:968-1016), with the activations the
+// backward pass needs.
+static int forward_logits(DeviceCtx *c, Model &m, const float *P, const int *tok) {
   const int N = m.N, D = m.D, F = m.F, KD = m.KD, V = m.V;
-  const size_t ND = (size_t)N * D, NF = (size_t)N * F;
+  const size_t NF = (size_t)N * F;
   const float *emb = P + m.o_emb;
-  // ---------------- forward (tinylm.c:968-1029)
   TRY(k_embed_fwd(c, emb, tok, m.a_in[0], N, D, V));
   for (int l = 0; l < m.L; l++) {
     float *xin = m.a_in[l];
@@ -137,17 +135,24 @@ static int micro_step(DeviceCtx *c, Model &m, const float *P, float *G, const in
   TRY(k_rmsnorm_fwd(c, m.x_final, P + m.o_nf, m.fn, m.fn_rinv, N, D));
   // tied head: logits = fn @ emb^T  (memset + mm_bt, 1015-1016, as one overwrite)
   TRY(gemm_add(c, GemmOp::NT, m.logits, m.fn, emb, N, V, D, nullptr));
-  // softmax + CE, logits gradient written in place (1019-1028, 1076-1082)
-  TRY(k_softmax_ce(c, m.logits, tgt, N, V, scale, m.loss_rows));
-  TRY(k_loss_sum(c, m.loss_rows, N, m.loss_acc));
-  if (!backward) return TL_OK;
+  return TL_OK;
+}
 
-  // ---------------- backward (tinylm.c:1072-1154)
+// The backward pass (tinylm.c:1072-1154) from the logits' gradient, which
+// stands in m.logits; gradients accumulate into G.  tgt_mtp: targets of the
+// MTP heads, each weighted by wk * scale (nullptr: the heads are left out).
+// ov (data-parallel step only, last micro-batch): told after each layer which
+// tail of G is final, so shard reductions start during the backward pass.
+static int backward_logits(DeviceCtx *c, Model &m, const float *P, float *G, const int *tok, const int *const *tgt_mtp,
+                           float scale, OverlapState *ov) {
+  const int N = m.N, D = m.D, F = m.F, KD = m.KD, V = m.V;
+  const size_t ND = (size_t)N * D, NF = (size_t)N * F;
+  const float *emb = P + m.o_emb;
   float *gemb = G + m.o_emb;
   TRY(gemm(c, GemmOp::NN, m.dfn, m.logits, emb, N, V, D));       // dfn = dlogits @ emb
   TRY(gemm(c, GemmOp::TN, gemb, m.logits, m.fn, N, V, D));        // dEmb += dlogits^T @ fn
   // MTP heads (1036-1069): hk = fn + silu(fn@Wk), tied logits, weight 0.2*0.8^k
-  for (int kh = 0; kh < m.n_mtp; kh++) {
+  for (int kh = 0; tgt_mtp && kh < m.n_mtp; kh++) {
     const float wk = 0.2f * powf(0.8f, (float)kh);
     const float *Wk = P + m.o_mtp[kh];
     TRY(gemm(c, GemmOp::NN, m.t1, m.fn, Wk, N, D, D));
@@ -202,6 +207,16 @@ static int micro_step(DeviceCtx *c, Model &m, const float *P, float *G, const in
   return TL_OK;
 }
 
+// One micro-batch: forward + backward, gradients accumulated into G.
+static int micro_step(DeviceCtx *c, Model &m, const float *P, float *G, const int *tok, const int *tgt,
+                      const int *const *tgt_mtp, float scale, bool backward, OverlapState *ov = nullptr) {
+  TRY(forward_logits(c, m, P, tok));
+  // softmax + CE, logits gradient written in place (1019-1028, 1076-1082)
+  TRY(k_softmax_ce(c, m.logits, tgt, m.N, m.V, scale, m.loss_rows));
+  TRY(k_loss_sum(c, m.loss_rows, m.N, m.loss_acc));
+  return backward ? backward_logits(c, m, P, G, tok, tgt_mtp, scale, ov) : TL_OK;
+}
+
 // The step's GEMMs run as one long sequence under the power cap: the
 // automatic engine choice gives them the hybrid split (gemm_sustained_scope).
 struct SustainedGemms {
@@ -222,6 +237,48 @@ static int run_batch(DeviceCtx *c, Model &m, const float *P, float *G, const int
     for (int kh = 0; kh < m.n_mtp; kh++) mt[kh] = tgt_mtp + (size_t)kh * Ntot + off;
     TRY(micro_step(c, m, P, G, tok + off, tgt + off, mt.data(), scale, backward,
                    i == B / m.mb - 1 ? ov : nullptr));
+  }
+  if (loss_dev) TRY(k_loss_final(c, m.loss_acc, (double)Ntot, loss_dev));
+  return TL_OK;
+}
+
+// A batch of rows scored (tl_model_score) or distilled (tl_model_distill_*),
+// micro-batch by micro-batch.
+static int check_batch(const Model &m, int B) {
+  if (B < 1 || B % m.mb) return set_error(TL_EINVAL, "batch %d must be a positive multiple of the micro-batch %d", B, m.mb);
+  return TL_OK;
+}
+
+static int score_batch(DeviceCtx *c, Model &m, const float *P, const int *tok, const int *tgt, int B, float temperature,
+                       float *logp, float *entropy, int K, int *top_ids, float *top_logp) {
+  SustainedGemms sustained;
+  const LogitRows z{m.logits, TL_F32, m.V, m.N, m.V};
+  for (int i = 0; i < B / m.mb; i++) {
+    const size_t off = (size_t)i * m.N;
+    TRY(forward_logits(c, m, P, tok + off));
+    TRY(k_token_logprobs(c, z, logp ? tgt + off : nullptr, temperature, logp ? logp + off : nullptr,
+                         entropy ? entropy + off : nullptr, nullptr, K, K ? top_ids + off * K : nullptr,
+                         K ? top_logp + off * K : nullptr));
+  }
+  return TL_OK;
+}
+
+static int distill_batch(DeviceCtx *c, Model &m, const float *P, float *G, const int *tok, const int *t_ids,
+                         const float *t_vals, int K, const float *weight, int B, float temperature, int tail,
+                         float *loss_dev) {
+  SustainedGemms sustained;
+  const size_t Ntot = (size_t)B * m.T;
+  const float scale = 1.0f / (float)Ntot;
+  const LogitRows z{m.logits, TL_F32, m.V, m.N, m.V};
+  TL_TRY_CUDA(cudaMemsetAsync(m.loss_acc, 0, sizeof(double), c->stream));
+  for (int i = 0; i < B / m.mb; i++) {
+    const size_t off = (size_t)i * m.N;
+    TRY(forward_logits(c, m, P, tok + off));
+    // the logits' gradient in their place
+    TRY(k_distill_topk(c, z, t_ids + off * K, t_vals + off * K, K, temperature, tail, weight ? weight + off : nullptr,
+                       scale, nullptr, m.loss_rows, G ? m.logits : nullptr, m.V));
+    TRY(k_loss_sum(c, m.loss_rows, m.N, m.loss_acc));
+    if (G) TRY(backward_logits(c, m, P, G, tok + off, nullptr, scale, nullptr));
   }
   if (loss_dev) TRY(k_loss_final(c, m.loss_acc, (double)Ntot, loss_dev));
   return TL_OK;
@@ -425,6 +482,65 @@ TL_API int tl_model_step(void *h, float *P, float *G, float *M, float *V, const 
   return launch_adamw(c, P, G, M, V, m->np, lr, 0.9f, 0.95f, 0.1f, t, 1.0f, gscale);  // 2633
 }
 
+
+TL_API int tl_model_score(void *h, const float *P, const int *tok, const int *tgt, int B, float temperature, float *logp,
+                          float *entropy, int K, int *top_ids, float *top_logp) {
+  Model *m = static_cast<Model *>(h);
+  if (!m) return set_error(TL_EINVAL, "NULL model");
+  TL_REQUIRE_CTX(c);
+  if (c->device != m->device) return set_error(TL_EINVAL, "model belongs to device %d", m->device);
+  int rc;
+  if ((rc = check_batch(*m, B)) || (rc = check_temperature(temperature)) || (rc = check_topk(K, m->V))) return rc;
+  if (m->V > TL_VOCAB_MAX) return set_error(TL_EINVAL, "V = %d above %d", m->V, TL_VOCAB_MAX);
+  if (!logp && !entropy && K == 0) return set_error(TL_EINVAL, "no output asked for");
+  if ((logp != nullptr) != (tgt != nullptr)) return set_error(TL_EINVAL, "tgt and logp come together");
+  if (K == 0 && (top_ids || top_logp)) return set_error(TL_EINVAL, "top_ids and top_logp take K >= 1");
+  if ((rc = check_ptr_here(c, P, "P", 4)) || (rc = check_ptr_here(c, tok, "tok", 4)) ||
+      (logp && ((rc = check_ptr_here(c, tgt, "tgt", 4)) || (rc = check_ptr_here(c, logp, "logp", 4)))) ||
+      (entropy && (rc = check_ptr_here(c, entropy, "entropy", 4))) ||
+      (K && ((rc = check_ptr_here(c, top_ids, "top_ids", 4)) || (rc = check_ptr_here(c, top_logp, "top_logp", 4)))))
+    return rc;
+  return score_batch(c, *m, P, tok, tgt, B, temperature, logp, entropy, K, top_ids, top_logp);
+}
+
+TL_API int tl_model_distill(void *h, const float *P, float *G, const int *tok, const int *t_ids, const float *t_vals,
+                            int K, const float *weight, int B, float temperature, int tail, float *loss_dev) {
+  Model *m = static_cast<Model *>(h);
+  if (!m) return set_error(TL_EINVAL, "NULL model");
+  TL_REQUIRE_CTX(c);
+  if (c->device != m->device) return set_error(TL_EINVAL, "model belongs to device %d", m->device);
+  int rc;
+  if ((rc = check_batch(*m, B)) || (rc = check_temperature(temperature)) || (rc = check_topk(K, m->V))) return rc;
+  if (m->V > TL_VOCAB_MAX) return set_error(TL_EINVAL, "V = %d above %d", m->V, TL_VOCAB_MAX);
+  if (K < 1) return set_error(TL_EINVAL, "K = 0: a teacher names at least one token");
+  if (tail != 0 && tail != 1) return set_error(TL_EINVAL, "tail %d is neither 0 nor 1", tail);
+  if (!G && !loss_dev) return set_error(TL_EINVAL, "no output asked for");
+  if ((rc = check_ptr_here(c, P, "P", 4)) || (rc = check_ptr_here(c, tok, "tok", 4)) ||
+      (rc = check_ptr_here(c, t_ids, "t_ids", 4)) || (rc = check_ptr_here(c, t_vals, "t_vals", 4)) ||
+      (G && (rc = check_ptr_here(c, G, "G", 4))) || (weight && (rc = check_ptr_here(c, weight, "weight", 4))) ||
+      (loss_dev && (rc = check_ptr_here(c, loss_dev, "loss_dev", 4))))
+    return rc;
+  return distill_batch(c, *m, P, G, tok, t_ids, t_vals, K, weight, B, temperature, tail, loss_dev);
+}
+
+TL_API int tl_model_distill_step(void *h, float *P, float *G, float *M, float *V, const int *tok, const int *t_ids,
+                                 const float *t_vals, int K, const float *weight, int B, float temperature, int tail,
+                                 float lr, int t, float max_norm, float *loss_dev, float *norm_dev) {
+  Model *m = static_cast<Model *>(h);
+  if (!m) return set_error(TL_EINVAL, "NULL model");
+  TL_REQUIRE_CTX(c);
+  if (t < 1) return set_error(TL_EINVAL, "step t must be >= 1 (got %d)", t);
+  int rc;
+  if ((rc = check_ptr_here(c, G, "G", 4)) || (rc = check_ptr_here(c, M, "M", 4)) || (rc = check_ptr_here(c, V, "V", 4)) ||
+      (norm_dev && (rc = check_ptr_here(c, norm_dev, "norm_dev", 4))))
+    return rc;
+  if (c->device != m->device) return set_error(TL_EINVAL, "model belongs to device %d", m->device);
+  TL_TRY_CUDA(cudaMemsetAsync(G, 0, sizeof(float) * m->np, c->stream));
+  if ((rc = tl_model_distill(h, P, G, tok, t_ids, t_vals, K, weight, B, temperature, tail, loss_dev))) return rc;
+  float *gscale = c->scalars + 1;
+  if ((rc = launch_sumsq(c, G, m->np, c->sumsq, norm_dev, gscale, max_norm))) return rc;
+  return launch_adamw(c, P, G, M, V, m->np, lr, 0.9f, 0.95f, 0.1f, t, 1.0f, gscale);
+}
 
 // One training step as a CUDA graph: captured on the first call (and again
 // whenever a buffer, the batch or max_norm changes), then replayed with one

@@ -90,6 +90,43 @@ class Model:
             None if loss_out is None else ops._ptr(loss_out, "loss_out", 1),
             None if norm_out is None else ops._ptr(norm_out, "norm_out", 1)))
 
+    def score(self, P, tok, tgt, B, logp, entropy=None, K=0, top_ids=None, top_logp=None, temperature=1.0):
+        """Per position of a batch: log p of the target token, the entropy and
+        the K most likely tokens (ops.token_logprobs on the model's logits).
+        tgt and logp may both be None; outputs left None are not computed."""
+        ops._prep(P)
+        n = B * self.T
+        check(lib().tl_model_score(
+            self.h, ops._ptr(P, "P", self.nparams), ops._vec(tok, "tok", n, torch.int32),
+            ops._vec(tgt, "tgt", n, torch.int32), B, temperature, ops._vec(logp, "logp", n),
+            ops._vec(entropy, "entropy", n), K, ops._vec(top_ids, "top_ids", n * K, torch.int32),
+            ops._vec(top_logp, "top_logp", n * K)))
+
+    def distill(self, P, G, tok, t_ids, t_vals, K, B, weight=None, temperature=1.0, tail=False, loss_out=None):
+        """G += gradient of the mean divergence from a teacher's K tokens a
+        position (ops.distill_topk on the model's logits, rows' losses over
+        B*T); G None gives the loss alone.  t_ids and t_vals are what score()
+        of the teacher wrote to top_ids and top_logp."""
+        ops._prep(P)
+        n = B * self.T
+        check(lib().tl_model_distill(
+            self.h, ops._ptr(P, "P", self.nparams), ops._vec(G, "G", self.nparams),
+            ops._vec(tok, "tok", n, torch.int32), ops._vec(t_ids, "t_ids", n * K, torch.int32),
+            ops._vec(t_vals, "t_vals", n * K), K, ops._vec(weight, "weight", n), B, temperature, int(tail),
+            ops._vec(loss_out, "loss_out", 1)))
+
+    def distill_step(self, P, G, M, V, tok, t_ids, t_vals, K, B, lr, t, weight=None, temperature=1.0, tail=False,
+                     max_norm=1.0, loss_out=None, norm_out=None):
+        """One training step on a teacher's tokens: distill() into a zeroed G,
+        clip, AdamW."""
+        ops._prep(P)
+        n, np_ = B * self.T, self.nparams
+        check(lib().tl_model_distill_step(
+            self.h, ops._ptr(P, "P", np_), ops._ptr(G, "G", np_), ops._ptr(M, "M", np_), ops._ptr(V, "V", np_),
+            ops._vec(tok, "tok", n, torch.int32), ops._vec(t_ids, "t_ids", n * K, torch.int32),
+            ops._vec(t_vals, "t_vals", n * K), K, ops._vec(weight, "weight", n), B, temperature, int(tail), lr, int(t),
+            max_norm, ops._vec(loss_out, "loss_out", 1), ops._vec(norm_out, "norm_out", 1)))
+
     def step_zero1(self, z, P, G, M_shard, V_shard, tok, tgt, tgt_mtp, B, lr, t, max_norm=1.0, loss_out=None,
                    norm_out=None):
         """Data-parallel step over the Zero1 communicator z (NCCL exchange),

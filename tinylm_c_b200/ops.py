@@ -37,7 +37,7 @@ def init(device=0):
 
 
 def _bind_stream(idx):
-    s = torch.cuda.current_stream(idx).cuda_stream
+    s = torch._C._cuda_getCurrentRawStream(idx)   # what torch.cuda.current_stream(idx).cuda_stream reads
     if _stream_set.get(idx) != s:
         check(lib().tl_set_stream(s))
         _stream_set[idx] = s
