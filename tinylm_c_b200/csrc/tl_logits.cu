@@ -8,30 +8,53 @@
 // H = log s - (1/s) sum e_v (z_v - m) / temperature.  Everything is taken
 // relative to the row's largest logit, so rows of a type's lowest value (every
 // token masked) and very large logits keep their distribution.
+#include <algorithm>
 #include <cmath>
 #include "tl_logits_dev.cuh"
 
 namespace tl {
 
+// The choices below, each with what it was measured against (B200, us; "scaled"
+// is 16384 x 8192 fp32, "50k" 4096 x 50000 bf16, "131k" N x 131072 bf16):
+//
+//  * A row longer than one piece of 2048 chunks is split over a cluster where
+//    there are no more rows than SMs: 131k scores with K = 20 take 8 instead of
+//    29 us for 1 row, 16 against 30 for 74 and 24 against 31 for 148, but 36
+//    against 35 for 296.  So many blocks a row that they fill the SMs once, two
+//    at least: 74 rows of 32768 fp32 take 5.6, 5.9 and 7.7 us with 2, 4 and 8.
+//    A row of one piece gains nothing from it (6.9 against 6.2 us for a
+//    distilled row of 8192 fp32).
+//  * Alternatives: pieces of 2048 chunks, one stage, 128 threads (5 blocks an
+//    SM): scaled K = 64 takes 205 us, with two stages (3 blocks) 235, with 256
+//    threads 272, with pieces of 1024 chunks and two stages 250.  Above K = 64
+//    four warps' maxima are too few for a threshold: K = 128 takes 496 us with
+//    256 threads and 2069 with 128.
+//  * No alternatives: pieces of 1024 chunks, two stages, 128 threads: 86 us
+//    scaled and 81 for 50k; one stage of 2048 and 256 threads 92 and 100.
+//  * Distillation: 256 threads, pieces of 2048 chunks, two stages: 207 us scaled
+//    with a tail (with one stage 224) and 104 for 2048 x 50000 fp16 (123).  Rows
+//    of six pieces or more, which come twice, three stages: so two blocks an SM,
+//    whose rows stay in L2 in between, 218 us for 2048 rows of 131k against 242.
+//  * Short rows, up to 256 chunks, have one computing warp, if its 32 maxima are
+//    enough for a threshold (K <= 16).
 RowPlan plan_rows(const DeviceCtx *c, const LogitRows &z, int K, bool twice) {
   const int es = z.dtype == TL_F32 ? 4 : 2, ev = 16 / es;
   // chunks of a row: its own alignment where all rows share it, else the worst
   const bool one = (z.ld * es) % 16 == 0 || z.N == 1;
   const int mis = one ? (int)(reinterpret_cast<uintptr_t>(z.p) & 15) / es : ev - 1;
   const int nch = (z.V + mis + ev - 1) / ev;
-  // few rows: several blocks a row
-  int blocks = 1;
-  while ((long long)z.N * blocks * 2 <= 4 * c->num_sms && blocks * 2 <= 8 && nch / blocks >= 512) blocks *= 2;
-  RowPlan p{256, blocks, {z.p, z.ld, z.N, z.V, nch, 1, 1, 0, 0}};
-  if (blocks > 1) {
-    if ((nch + blocks - 1) / blocks > 6144) blocks = p.blocks = (nch + 6143) / 6144;
-    p.l.per = (nch + blocks - 1) / blocks;
-    p.l.pieces = blocks;
+  constexpr int kPiece = 2048, kMostPerBlock = 6144;           // of a cluster: 96 KB in one stage
+  RowPlan p{256, 1, {z.p, z.ld, z.N, z.V, nch, 1, 1, 0, 0}};
+  if (nch > kPiece && z.N <= c->num_sms) {
+    p.blocks = 2;
+    while (z.N * p.blocks * 2 <= c->num_sms && p.blocks < 8) p.blocks *= 2;
+    p.blocks = std::max(p.blocks, (nch + kMostPerBlock - 1) / kMostPerBlock);
+    p.l.per = (nch + p.blocks - 1) / p.blocks;
+    p.l.pieces = p.blocks;
     p.threads = p.l.per <= 512 ? 128 : p.l.per <= 2048 ? 256 : 512;
   } else {
     p.threads = nch <= 256 && K <= 16 ? 32 : nch <= 1024 ? 128 : twice || K > 64 ? 256 : 128;
-    const int per = twice || K > 0 ? 2048 : 1024;
-    p.l.per = nch < per ? nch : per;
+    p.l.per = std::min(nch, twice || K > 0 ? kPiece : kPiece / 2);
     p.l.pieces = (nch + p.l.per - 1) / p.l.per;
     p.l.stages = p.threads == 32 ? 4 : !twice && K > 0 ? 1 : twice && p.l.pieces >= 6 ? 3 : 2;
   }
