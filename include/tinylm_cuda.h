@@ -231,7 +231,8 @@ int tl_model_step_zero1(void *handle, float *P, float *G, float *M_shard, float 
 /* ------------------------------------------- vocabulary rows (logits) */
 /* Operators over rows of logits: N rows of V values, row n at logits + n*ld
  * elements (ld >= V, any alignment of the element type), of `dtype` TL_F32,
- * TL_BF16 or TL_F16.  N >= 0 (0: nothing is done), 1 <= V <= TL_VOCAB_MAX,
+ * TL_BF16 or TL_F16.  0 <= N <= 2^30 (0: nothing is done), 1 <= V <=
+ * TL_VOCAB_MAX,
  * 1e-6 <= temperature <= 1e6.  With y = z/temperature:
  *   log p_v = y_v - log sum_u exp(y_u),   H = -sum_v p_v log p_v.
  * Sums, statistics and every float output are fp32 whatever the logits' type.

@@ -20,7 +20,7 @@ def distill(dtype=0, ld=100, K=4, N=2, V=100, tau=1.0, tail=0, scale=1.0, loss=P
     return _lib.lib().tl_distill_topk(P, dtype, ld, P, P, K, N, V, tau, tail, None, scale, loss, dz, ldd)
 
 
-ROWS = [dict(dtype=3), dict(dtype=-1), dict(N=-1), dict(V=0), dict(V=-5), dict(V=_lib.TL_VOCAB_MAX + 1, ld=1 << 20),
+ROWS = [dict(dtype=3), dict(dtype=-1), dict(N=-1), dict(N=(1 << 30) + 1), dict(V=0), dict(V=-5), dict(V=_lib.TL_VOCAB_MAX + 1, ld=1 << 20),
         dict(ld=99), dict(ld=-1), dict(ld=1 << 41), dict(tau=0.0), dict(tau=-1.0), dict(tau=float("nan")),
         dict(tau=float("inf")), dict(tau=1e-7), dict(tau=1e7)]
 
@@ -84,6 +84,36 @@ def test_binding_refuses_tensors_it_cannot_take():
         ops.token_logprobs(z, i, -1, 8, e)
     with pytest.raises(ValueError, match="bad sizes"):
         ops.distill_topk(z, i, e, 2, 0, 1, e, z)
+
+
+def test_calls_run_on_the_tensor_s_device(monkeypatch):
+    """Tensors of another device than the current one: the call is made with theirs current."""
+    seen, current = [], [0]
+
+    class On:
+        def __init__(self, d):
+            self.d = d
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.d
+
+        def __exit__(self, *a):
+            current[0] = self.before
+
+    class Lib:
+        def tl_token_logprobs(self, *a):
+            seen.append(current[0])
+            return 0
+
+    t = type("T", (), {"device": type("D", (), {"index": 1})()})()
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", lambda d: On(d.index))
+    monkeypatch.setattr(ops, "_prep", lambda t: seen.append(("prep", current[0])))
+    monkeypatch.setattr(ops, "lib", Lib)
+    ops._call_on(t, "tl_token_logprobs")
+    current[0] = 1
+    ops._call_on(t, "tl_token_logprobs")
+    assert seen == [("prep", 1), 1, ("prep", 1), 1] and current[0] == 1
 
 
 class Fake(torch.Tensor):

@@ -493,6 +493,118 @@ def test_same_bits_twice_captured_and_on_two_streams(cuda, N, V):
             assert all(torch.equal(w[k], o[k]) for k in w)
 
 
+@pytest.mark.parametrize("tau", [1e-6, 0.03, 50.0, 1e6])
+def test_extreme_temperatures(cuda, tau):
+    """Close to the largest logit alone, and close to uniform."""
+    rng = np.random.default_rng(6)
+    for N, V, dtype in ((4, 3000, "f32"), (2, 40000, "bf16")):
+        z, _ = make(rng, N, V, dtype)
+        ids = random_ids(rng, N, V)
+        check_score(z, ids, 10, tau)
+        H, stats = scored(z, ids, tau)
+        a = torch.ones(N, device="cuda")
+        want, tol = ref.score_grad(f64(z), ids.cpu().numpy(), tau, f64(a), None, dtype)
+        dz = torch.empty_like(z)
+        ops.token_logprobs_bwd(dz, z, ids, N, V, stats, a, temperature=tau)
+        ref.close(dz.cpu().double(), want, tol, "dlogits")
+        t_ids, t_vals = teacher(rng, z, 6, tau, False)
+        L, lt, d, dt = ref.distill(f64(z), t_ids, t_vals, tau, False, None, tau, dtype)
+        loss = run_distill(z, t_ids, t_vals, tau, False, None, tau, dz)
+        ref.close(loss.cpu(), L, lt, "loss")
+        ref.close(dz.cpu().double(), d, dt, "dlogits")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_many_rows_of_hard_patterns(cuda, dtype):
+    """Rows that overflow the list of candidates beside rows that do not, many to a block, for every
+    way the rows are laid out: short, one piece, several pieces."""
+    rng = np.random.default_rng(8)
+    for N, V, K in ((1500, 300, 12), (1300, 6000, 40), (700, 20000, 128), (400, 70000, 5)):
+        z, _ = make(rng, N, V, dtype)
+        names = ["constant", "ascending", "lowest_mask", "inf_mask", "empty", "mass_ties", "two_values"]
+        rows = {name: torch.from_numpy(pattern(name, rng, V, dtype)).to(z) for name in names}
+        some = rng.choice(N, 70, replace=False)
+        for i, n in enumerate(some):
+            z[n] = rows[names[i % len(names)]]
+        ids = random_ids(rng, N, V)
+        logp, H, stats, ti, tl = run_score(z, ids, K, 1.0)
+        pick = np.concatenate([some, rng.choice(N, 40, replace=False)])
+        at = torch.from_numpy(pick).cuda()
+        want = ref.score(f64(z[at]), ids[at].cpu().numpy(), 1.0, K)
+        ref.close(logp[at].cpu(), want["logp"], want["logp_tol"], "logp")
+        ref.close(H[at].cpu(), want["entropy"], want["entropy_tol"], "entropy")
+        assert np.array_equal(ti[at].cpu().numpy(), want["top_ids"])
+        ref.close(tl[at].cpu(), want["top_logp"], want["top_logp_tol"], "top_logp")
+
+
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill_many_rows(cuda, tail):
+    """Many rows to a block, every third without weight, in one piece and in several, in place."""
+    rng = np.random.default_rng(13)
+    for N, V, K, dtype, pad in ((1400, 700, 5, "f32", 1), (1200, 8192, 20, "f32", 0), (500, 50001, 9, "bf16", 0),
+                                (460, 120000, 6, "bf16", 8)):
+        z, flat = make(rng, N, V, dtype, pad)
+        pick = np.sort(rng.choice(N, 30, replace=False))
+        at = torch.from_numpy(pick).cuda()
+        t = z.float() + torch.randn(N, V, device="cuda")
+        vals, ids = torch.topk(t, K, dim=1)
+        if tail:
+            vals = torch.log_softmax(t, 1).gather(1, ids)
+        ids, vals = ids.int().contiguous(), vals.contiguous()
+        w = torch.rand(N, device="cuda") + 0.5
+        w[::3] = 0.0
+        L, lt, d, dt = ref.distill(f64(z[at]), ids[at].cpu().numpy(), vals[at].cpu().numpy(), 1.0, tail, f64(w[at]), 2.0,
+                                   dtype)
+        loss = torch.empty(N, device="cuda")
+        dz = torch.full_like(z, 5.0)
+        ops.distill_topk(z, ids, vals, N, V, K, loss, dz, weight=w, scale=2.0, tail=tail)
+        ref.close(loss[at].cpu(), L, lt, "loss")
+        ref.close(dz[at].cpu().double(), d, dt, "dlogits")
+        assert (dz[::3] == 0).all() and (loss[::3] == 0).all()
+        again = torch.empty(N, device="cuda")
+        keep = flat.clone()
+        ops.distill_topk(z, ids, vals, N, V, K, again, z, weight=w, scale=2.0, tail=tail)
+        assert torch.equal(again, loss) and torch.equal(z, dz)
+        keep[:N * (V + pad)].view(N, V + pad)[:, :V] = z
+        assert torch.equal(flat, keep)
+
+
+def test_first_call_inside_a_capture():
+    """In a fresh process, after ops.init, the first call of each operator is captured."""
+    import subprocess
+    import sys
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device visible")
+    code = """
+import torch
+from tinylm_c_b200 import ops
+ops.init(0)
+for N, V in ((3, 900), (2, 70000), (300, 9000)):
+    z = torch.randn(N, V, device="cuda"); ids = torch.zeros(N, dtype=torch.int32, device="cuda")
+    lp, H, st = torch.zeros(N, device="cuda"), torch.zeros(N, device="cuda"), torch.zeros(N, 2, device="cuda")
+    ti, tl = torch.zeros(N, 4, dtype=torch.int32, device="cuda"), torch.zeros(N, 4, device="cuda")
+    dz, L = torch.zeros_like(z), torch.zeros(N, device="cuda")
+    def go():
+        ops.token_logprobs(z, ids, N, V, lp, entropy=H, stats=st, K=4, top_ids=ti, top_logp=tl)
+        ops.distill_topk(z, ti, tl, N, V, 4, L, dz, tail=True)
+        ops.token_logprobs_bwd(dz, z, ids, N, V, st, lp, entropy=H, dentropy=H)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        go()
+    g.replay(); torch.cuda.synchronize()
+    got = [t.clone() for t in (lp, H, ti, tl, L, dz)]
+    for t in (lp, H, ti, tl, L, dz): t.zero_()
+    go(); torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, (lp, H, ti, tl, L, dz)))
+    assert torch.allclose(lp, torch.log_softmax(z, 1)[:, 0], atol=1e-4)
+print("captured")
+"""
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
 def test_offsets_past_32_bits(cuda):
     """Rows that start more than 2^32 bytes and 2^31 elements into the logits."""
     N, V, pad = 3, 5000, (1 << 30) + 1001

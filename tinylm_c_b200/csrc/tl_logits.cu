@@ -140,8 +140,8 @@ size_t dtype_size(int dtype) { return dtype == TL_F32 ? 4 : 2; }
 int check_rows(int dtype, long long ld, int N, int V, const char *what) {
   if (dtype != TL_F32 && dtype != TL_BF16 && dtype != TL_F16)
     return set_error(TL_EINVAL, "dtype %d is none of TL_F32, TL_BF16, TL_F16", dtype);
-  if (N < 0 || V < 1 || V > TL_VOCAB_MAX)
-    return set_error(TL_EINVAL, "N = %d, V = %d: N >= 0 and 1 <= V <= %d are taken", N, V, TL_VOCAB_MAX);
+  if (N < 0 || N > (1 << 30) || V < 1 || V > TL_VOCAB_MAX)
+    return set_error(TL_EINVAL, "N = %d, V = %d: 0 <= N <= 2^30 and 1 <= V <= %d are taken", N, V, TL_VOCAB_MAX);
   if (ld < V || ld > (1LL << 40)) return set_error(TL_EINVAL, "row stride of %s %lld below V = %d", what, ld, V);
   return TL_OK;
 }
