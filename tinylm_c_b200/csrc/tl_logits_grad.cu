@@ -424,7 +424,6 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) distill_kernel(c
   const Rows<T> t(a.l);
   const int N = a.l.N, stride = (int)gridDim.x, first_row = (int)blockIdx.x, stages = a.l.stages, pieces = a.l.pieces;
   const int passes = a.dz && pieces > 1 ? 2 : 1;
-  const bool made_ready = TAIL || t.ragged;
   void *const entries = s_dyn + (size_t)stages * a.l.chunks * 16;
   const Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), stages, a.l.chunks, s_full, &s_abort, a.err};
   if (tid == 0) {
@@ -479,13 +478,10 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) distill_kernel(c
         s_weight[flip] = w;
         tc::mbar_arrive(tc::smem_u32(&s_taught[flip]));
       }
-      for (int i = 0; made_ready && w != 0.0f && i < passes * pieces; i++) {
+      for (int i = 0; TAIL && w != 0.0f && i < passes * pieces; i++) {
         pipe.wait(&s_full[get.s], get.phase);
-        if (i < pieces) {                          // the second time the named tokens are written over anyway
-          const Piece<T> pc(t, n, i);
-          if (TAIL) take_out(pc, reinterpret_cast<T *>(pipe.stage(get.s)), l);
-          if (t.ragged) pc.mask_ends(pipe.stage(get.s), [&](int) { return lane == 0; });
-        }
+        // the second time the named tokens are written over anyway
+        if (i < pieces) take_out(Piece<T>(t, n, i), reinterpret_cast<T *>(pipe.stage(get.s)), l);
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_ready[get.s]));
         get.next(stages);
@@ -497,7 +493,7 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) distill_kernel(c
   Turn turn;
   auto arrived = [&] {
     pipe.wait(&s_full[turn.s], turn.phase);
-    if (made_ready) pipe.wait(&s_ready[turn.s], turn.phase);
+    if (TAIL) pipe.wait(&s_ready[turn.s], turn.phase);
   };
   auto done = [&] {
     __syncwarp();
@@ -522,6 +518,7 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) distill_kernel(c
       Running run;
       for (int i = 0; i < pieces; i++) {
         arrived();
+        if (t.ragged) Piece<T>(t, n, i).mask_ends(pipe.stage(turn.s), [&](int k) { return k % TH == tid; });
         add_share<T, TH, false>(run, tc::smem_u32(pipe.stage(turn.s)), max(0, min(r.n - i * t.per, t.per)), a.c);
         if (pieces > 1 || !a.dz) done();
       }

@@ -20,7 +20,7 @@
 namespace tl {
 namespace lg {
 
-constexpr int CAP = 512;             // candidates a row's first block holds
+constexpr int CAP = 512;             // candidates a cluster's first block holds, and one block's row at most
 
 // Order of the alternatives as one integer: larger logit first, then the
 // lower index.  x + 0 makes -0 equal to +0.
@@ -180,7 +180,7 @@ struct ScoreArgs {
   const int *ids;
   float c, inv_t;                    // log2(e) / temperature, 1 / temperature
   float *logp, *entropy, *stats;
-  int K, j, g_full, updates;         // alternatives; see threshold() for the others
+  int K, j, g_full, updates, cap;    // alternatives; see threshold() for the others
   int *top_ids;
   float *top_logp;
   int *err;
@@ -351,8 +351,8 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) score_cluster_kernel(const
 // (elsewhere they cannot be among the K: the K elements at or above it come
 // earlier).  A threshold of the whole row then leaves few to put in order.
 
-// The K largest keys of a row in memory (up to CAP with them), where more than
-// CAP elements passed: at least K are at or above thr, or thr = -inf.  By TH
+// The K largest keys of a row in memory (up to cap with them), where more than
+// cap elements passed: at least K are at or above thr, or thr = -inf.  By TH
 // threads (barrier 1), over the row in L2: one pass counts the elements at or
 // above the threshold and those above it.  Few enough are collected (the
 // row's last threshold is higher than those that filled the list); fewer than
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) score_cluster_kernel(const
 // taken in order of their index; else the K-th largest value is searched, two
 // bits a pass.
 template <typename T, int TH>
-__device__ __noinline__ void select_row(const T *row, int V, int K, float thr, uint2 *keys, unsigned *s_count) {
+__device__ __noinline__ void select_row(const T *row, int V, int K, float thr, uint2 *keys, unsigned *s_count, int cap) {
   constexpr int EV = Elem<T>::EV, W = TH / 32;
   __shared__ int s_cnt[2][3][W];
   const Chunks<T> r(row, V);
@@ -412,7 +412,7 @@ __device__ __noinline__ void select_row(const T *row, int V, int K, float thr, u
   unsigned lo = order_of(thr == -INFINITY ? -FLT_MAX : thr), hi = order_of(INFINITY);
   int sum[3], above = 0;
   at_least(lo, lo + 1, hi, sum);
-  const bool few = sum[0] <= CAP;
+  const bool few = sum[0] <= cap;
   if (few) {
     hi = lo;                         // all of order lo or above are collected
     above = sum[0];
@@ -483,49 +483,39 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
   __shared__ Part s_part[2][W];
   __shared__ float s_thr[2], s_w[2][W];
   __shared__ unsigned short s_list[TOP ? W : 1][LIST];
-  __shared__ unsigned s_count[2];
-  __shared__ uint64_t s_full[MAX_STAGES], s_ready[MAX_STAGES], s_free[MAX_STAGES], s_done[2], s_taken[2];
+  __shared__ unsigned s_count;
+  __shared__ uint64_t s_full[MAX_STAGES], s_free[MAX_STAGES], s_done[2], s_taken[2], s_clear;
   __shared__ int s_abort;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Rows<T> t(a.l);
   const int N = a.l.N, stride = (int)gridDim.x, first_row = (int)blockIdx.x, stages = a.l.stages, pieces = a.l.pieces;
   const Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), stages, a.l.chunks, s_full, &s_abort, a.err};
-  uint2 *s_keys = reinterpret_cast<uint2 *>(s_dyn + (size_t)stages * a.l.chunks * 16);     // [2][CAP]
+  uint2 *keys = reinterpret_cast<uint2 *>(s_dyn + (size_t)stages * a.l.chunks * 16);       // [a.cap]
   if (tid == 0) {
     for (int i = 0; i < stages; i++) {
       tc::mbar_init(tc::smem_u32(&s_full[i]), 1);
-      tc::mbar_init(tc::smem_u32(&s_ready[i]), 1);
       tc::mbar_init(tc::smem_u32(&s_free[i]), W);
     }
     for (int i = 0; i < 2; i++) {
       tc::mbar_init(tc::smem_u32(&s_done[i]), W);
       tc::mbar_init(tc::smem_u32(&s_taken[i]), 1);
-      s_count[i] = 0;
     }
+    tc::mbar_init(tc::smem_u32(&s_clear), 1);
+    s_count = 0;
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
   if (warp == W) {                   // ---- the pieces
-    Turn put, get;
-    int gn = first_row, gi = 0, k = 0;             // the piece to be made ready
-    auto make_ready = [&] {
-      pipe.wait(&s_full[get.s], get.phase);
-      Piece<T>(t, gn, gi).mask_ends(pipe.stage(get.s), [&](int) { return lane == 0; });
-      if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_ready[get.s]));
-      get.next(stages);
-      if (++gi == pieces) { gi = 0; gn += stride; }
-    };
+    Turn put;
+    int k = 0;
     for (int n = first_row; n < N; n += stride)
       for (int i = 0; i < pieces; i++, k++) {
         if (k >= stages) pipe.wait(&s_free[put.s], put.phase ^ 1);
         if (lane == 0) pipe.issue(t, n, i, put.s, true, l2_once());
         __syncwarp();
         put.next(stages);
-        if (t.ragged && k >= stages - 1) make_ready();
       }
-    if (t.ragged)
-      while (gn < N) make_ready();
     return;
   }
   if (warp == W + 1) {               // ---- the results
@@ -556,9 +546,8 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
         }
       }
       if (TOP) {
-        const int found = bad ? 0 : (int)s_count[flip];
+        const int found = bad ? 0 : (int)s_count;
         const float thr = s_thr[flip];
-        uint2 *keys = s_keys + flip * CAP;
         int *to_id = a.top_ids + (size_t)n * a.K;
         float *to_lp = a.top_logp + (size_t)n * a.K;
         int got = 0;                 // the candidates at or above the last threshold, to the front
@@ -580,16 +569,25 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
           to_id[place] = (int)(0xFFFFFFFFu - (unsigned)k);
           to_lp[place] = (value_of(k) - p.m) * a.inv_t - ls;
         };
+        auto clear = [&] {           // the list has been read: the next row's
+          __syncwarp();
+          if (lane == 0) {
+            s_count = 0;
+            tc::mbar_arrive(tc::smem_u32(&s_clear));
+          }
+        };
         auto in_order = [&](auto &k) {
           constexpr int R = sizeof(k) / sizeof(k[0]);
 #pragma unroll
           for (int r = 0; r < R; r++) k[r] = key(lane + 32 * r);
+          clear();
           sort_keys<R>(k);
 #pragma unroll
           for (int r = 0; r < R; r++) put(lane * R + r, k[r]);
         };
         if (got <= 16) {
           const unsigned long long k = key(lane);
+          clear();
           int place = 0;
           for (int q = 0; q < got; q++) place += __shfl_sync(FULL, k, q) > k;
           put(place, k);
@@ -610,8 +608,6 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
           to_id[i] = -1;
           to_lp[i] = bad ? NAN : -INFINITY;
         }
-        __syncwarp();
-        if (lane == 0) s_count[flip] = 0;
       }
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_taken[flip]));
@@ -628,7 +624,6 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
     // this row's places in shared memory: the results' warp has taken the row before last from them
     if (count_rows >= 2) pipe.wait(&s_taken[flip], ((count_rows >> 1) - 1) & 1);
     const Chunks<T> r = t.row(n);
-    uint2 *keys = s_keys + flip * CAP;
     Running run;
     float thr = TOP && a.j ? INFINITY : -INFINITY;
     Passing pass{s_list[TOP ? warp : 0]};
@@ -645,24 +640,31 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
       }
       return w;
     };
+    // The list belongs to this row once the one before has been read from it.
+    bool mine = !TOP || count_rows == 0;
+    auto take_list = [&] {
+      if (!mine) pipe.wait(&s_clear, (count_rows - 1) & 1);
+      mine = true;
+    };
     for (int i = 0; i < pieces; i++) {
       const int c0 = i * t.per, cnt = max(0, min(r.n - c0, t.per));
       const uint32_t st = tc::smem_u32(pipe.stage(turn.s));
       bool equal = false;
       auto flush = [&] {
         pass.elements<T>(reinterpret_cast<const T *>(pipe.stage(turn.s)), thr, equal, [&](float f, int v) {
-          const unsigned at = atomicAdd(&s_count[flip], 1u);
-          if (at < CAP) keys[at] = make_uint2(__float_as_uint(f), (unsigned)(r.first(c0) + v));
+          const unsigned at = atomicAdd(&s_count, 1u);
+          if (at < (unsigned)a.cap) keys[at] = make_uint2(__float_as_uint(f), (unsigned)(r.first(c0) + v));
         });
       };
       pipe.wait(&s_full[turn.s], turn.phase);
-      if (t.ragged) pipe.wait(&s_ready[turn.s], turn.phase);
+      if (t.ragged) Piece<T>(t, n, i).mask_ends(pipe.stage(turn.s), [&](int k) { return k % TH == tid; });
       if (!TOP) {
         add_share<T, TH, ENT>(run, st, cnt, a.c);
       } else if (a.j && (i & (i + 1)) == 0 && i + 1 < 2 * a.updates) {
         add_share<T, TH, ENT>(run, st, cnt, a.c);
         thr = threshold();
         equal = true;
+        take_list();
         for_chunks<T, TH>(st, cnt, [&](const uint4 (&x)[4], int k) {
           float m[4];
 #pragma unroll
@@ -679,6 +681,7 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
           if (pass.n > LIST - 4 * 32) flush();
         });
       } else {
+        take_list();
         for_chunks<T, TH>(st, cnt, [&](const uint4 (&x)[4], int k) {
           const float m = run.add<T, ENT>(x, a.c);
           if (__any_sync(FULL, m > thr)) {
@@ -702,10 +705,10 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
       if (a.j && pieces > 1) thr = fmaxf(thr, threshold());
       if (tid == 0) s_thr[flip] = thr;
       bar_sync<TH>();
-      if (s_count[flip] > CAP) {
+      if (s_count > (unsigned)a.cap) {
         p = join_all<false>(s_part[flip], W, a.c);
         if (p.s >= 0.0f)             // a row without a distribution has no alternatives
-          select_row<T, TH>(r.row, t.V, a.K, thr, keys, &s_count[flip]);
+          select_row<T, TH>(r.row, t.V, a.K, thr, keys, &s_count, a.cap);
       }
     }
     __syncwarp();
@@ -724,7 +727,7 @@ template <typename T, int TH, bool ENT> int launch_cluster(DeviceCtx *c, const R
 }
 template <typename T, int TH, bool ENT, bool TOP> int launch_score(DeviceCtx *c, const RowPlan &pl, lg::ScoreArgs a) {
   static Resident seen[kMaxDevices];
-  return launch_rows((const void *)lg::score_kernel<T, TH, ENT, TOP>, c, pl, 64, TOP ? 2 * lg::CAP * 8 : 0,
+  return launch_rows((const void *)lg::score_kernel<T, TH, ENT, TOP>, c, pl, 64, TOP ? a.cap * 8 : 0,
                      &seen[c->device], &a);
 }
 template <typename T, bool ENT, bool TOP> int score_rows(DeviceCtx *c, const RowPlan &pl, const lg::ScoreArgs &a) {
@@ -751,6 +754,7 @@ void threshold(const RowPlan &pl, int ev, lg::ScoreArgs *a) {
   a->g_full = full;
   // of random logits 2 to 2.5 K of a threshold's part of the row pass, as many
   // again of each further part of that length: kept below 256
+  a->cap = a->K <= 64 ? 320 : lg::CAP;
   a->updates = std::max(1, (a->K * a->l.pieces + 99) / 100);
   a->j = 0;
   if (!a->K || !full) return;
@@ -765,7 +769,7 @@ int k_token_logprobs(DeviceCtx *c, const LogitRows &z, const int *ids, float tem
                      float *entropy, float *stats, int K, int *top_ids, float *top_logp) {
   TraceScope ts(c, "k_token_logprobs");
   const RowPlan pl = plan_rows(c, z, K, false);
-  lg::ScoreArgs a{pl.l, ids, lg::LOG2E / temperature, 1.0f / temperature, logp, entropy, stats, K, 0, 0, 0, top_ids,
+  lg::ScoreArgs a{pl.l, ids, lg::LOG2E / temperature, 1.0f / temperature, logp, entropy, stats, K, 0, 0, 0, 0, top_ids,
                   top_logp, c->err_flag};
   threshold(pl, z.dtype == TL_F32 ? 4 : 8, &a);
   if (z.dtype == TL_F32) return entropy ? score_typed<float, true>(c, pl, a) : score_typed<float, false>(c, pl, a);
