@@ -483,14 +483,14 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
   __shared__ Part s_part[2][W];
   __shared__ float s_thr[2], s_w[2][W];
   __shared__ unsigned short s_list[TOP ? W : 1][LIST];
-  __shared__ unsigned s_count;
-  __shared__ uint64_t s_full[MAX_STAGES], s_free[MAX_STAGES], s_done[2], s_taken[2], s_clear;
+  __shared__ unsigned s_count[2];
+  __shared__ uint64_t s_full[MAX_STAGES], s_free[MAX_STAGES], s_done[2], s_taken[2];
   __shared__ int s_abort;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Rows<T> t(a.l);
   const int N = a.l.N, stride = (int)gridDim.x, first_row = (int)blockIdx.x, stages = a.l.stages, pieces = a.l.pieces;
   const Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), stages, a.l.chunks, s_full, &s_abort, a.err};
-  uint2 *keys = reinterpret_cast<uint2 *>(s_dyn + (size_t)stages * a.l.chunks * 16);       // [a.cap]
+  uint2 *s_keys = reinterpret_cast<uint2 *>(s_dyn + (size_t)stages * a.l.chunks * 16);     // [2][a.cap]
   if (tid == 0) {
     for (int i = 0; i < stages; i++) {
       tc::mbar_init(tc::smem_u32(&s_full[i]), 1);
@@ -499,9 +499,8 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
     for (int i = 0; i < 2; i++) {
       tc::mbar_init(tc::smem_u32(&s_done[i]), W);
       tc::mbar_init(tc::smem_u32(&s_taken[i]), 1);
+      s_count[i] = 0;
     }
-    tc::mbar_init(tc::smem_u32(&s_clear), 1);
-    s_count = 0;
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -546,8 +545,9 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
         }
       }
       if (TOP) {
-        const int found = bad ? 0 : (int)s_count;
+        const int found = bad ? 0 : (int)s_count[flip];
         const float thr = s_thr[flip];
+        uint2 *keys = s_keys + flip * a.cap;
         int *to_id = a.top_ids + (size_t)n * a.K;
         float *to_lp = a.top_logp + (size_t)n * a.K;
         int got = 0;                 // the candidates at or above the last threshold, to the front
@@ -569,25 +569,16 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
           to_id[place] = (int)(0xFFFFFFFFu - (unsigned)k);
           to_lp[place] = (value_of(k) - p.m) * a.inv_t - ls;
         };
-        auto clear = [&] {           // the list has been read: the next row's
-          __syncwarp();
-          if (lane == 0) {
-            s_count = 0;
-            tc::mbar_arrive(tc::smem_u32(&s_clear));
-          }
-        };
         auto in_order = [&](auto &k) {
           constexpr int R = sizeof(k) / sizeof(k[0]);
 #pragma unroll
           for (int r = 0; r < R; r++) k[r] = key(lane + 32 * r);
-          clear();
           sort_keys<R>(k);
 #pragma unroll
           for (int r = 0; r < R; r++) put(lane * R + r, k[r]);
         };
         if (got <= 16) {
           const unsigned long long k = key(lane);
-          clear();
           int place = 0;
           for (int q = 0; q < got; q++) place += __shfl_sync(FULL, k, q) > k;
           put(place, k);
@@ -608,6 +599,8 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
           to_id[i] = -1;
           to_lp[i] = bad ? NAN : -INFINITY;
         }
+        __syncwarp();
+        if (lane == 0) s_count[flip] = 0;
       }
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_taken[flip]));
@@ -624,6 +617,7 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
     // this row's places in shared memory: the results' warp has taken the row before last from them
     if (count_rows >= 2) pipe.wait(&s_taken[flip], ((count_rows >> 1) - 1) & 1);
     const Chunks<T> r = t.row(n);
+    uint2 *keys = s_keys + flip * a.cap;
     Running run;
     float thr = TOP && a.j ? INFINITY : -INFINITY;
     Passing pass{s_list[TOP ? warp : 0]};
@@ -640,19 +634,13 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
       }
       return w;
     };
-    // The list belongs to this row once the one before has been read from it.
-    bool mine = !TOP || count_rows == 0;
-    auto take_list = [&] {
-      if (!mine) pipe.wait(&s_clear, (count_rows - 1) & 1);
-      mine = true;
-    };
     for (int i = 0; i < pieces; i++) {
       const int c0 = i * t.per, cnt = max(0, min(r.n - c0, t.per));
       const uint32_t st = tc::smem_u32(pipe.stage(turn.s));
       bool equal = false;
       auto flush = [&] {
         pass.elements<T>(reinterpret_cast<const T *>(pipe.stage(turn.s)), thr, equal, [&](float f, int v) {
-          const unsigned at = atomicAdd(&s_count, 1u);
+          const unsigned at = atomicAdd(&s_count[flip], 1u);
           if (at < (unsigned)a.cap) keys[at] = make_uint2(__float_as_uint(f), (unsigned)(r.first(c0) + v));
         });
       };
@@ -664,7 +652,6 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
         add_share<T, TH, ENT>(run, st, cnt, a.c);
         thr = threshold();
         equal = true;
-        take_list();
         for_chunks<T, TH>(st, cnt, [&](const uint4 (&x)[4], int k) {
           float m[4];
 #pragma unroll
@@ -681,7 +668,6 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
           if (pass.n > LIST - 4 * 32) flush();
         });
       } else {
-        take_list();
         for_chunks<T, TH>(st, cnt, [&](const uint4 (&x)[4], int k) {
           const float m = run.add<T, ENT>(x, a.c);
           if (__any_sync(FULL, m > thr)) {
@@ -705,10 +691,10 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
       if (a.j && pieces > 1) thr = fmaxf(thr, threshold());
       if (tid == 0) s_thr[flip] = thr;
       bar_sync<TH>();
-      if (s_count > (unsigned)a.cap) {
+      if (s_count[flip] > (unsigned)a.cap) {
         p = join_all<false>(s_part[flip], W, a.c);
         if (p.s >= 0.0f)             // a row without a distribution has no alternatives
-          select_row<T, TH>(r.row, t.V, a.K, thr, keys, &s_count, a.cap);
+          select_row<T, TH>(r.row, t.V, a.K, thr, keys, &s_count[flip], a.cap);
       }
     }
     __syncwarp();
@@ -727,7 +713,7 @@ template <typename T, int TH, bool ENT> int launch_cluster(DeviceCtx *c, const R
 }
 template <typename T, int TH, bool ENT, bool TOP> int launch_score(DeviceCtx *c, const RowPlan &pl, lg::ScoreArgs a) {
   static Resident seen[kMaxDevices];
-  return launch_rows((const void *)lg::score_kernel<T, TH, ENT, TOP>, c, pl, 64, TOP ? a.cap * 8 : 0,
+  return launch_rows((const void *)lg::score_kernel<T, TH, ENT, TOP>, c, pl, 64, TOP ? 2 * a.cap * 8 : 0,
                      &seen[c->device], &a);
 }
 template <typename T, bool ENT, bool TOP> int score_rows(DeviceCtx *c, const RowPlan &pl, const lg::ScoreArgs &a) {
