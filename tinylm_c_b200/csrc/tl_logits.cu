@@ -26,9 +26,9 @@ namespace tl {
 //    distilled row of 8192 fp32).
 //  * Alternatives: pieces of 2048 chunks, one stage, 128 threads (5 blocks an
 //    SM): scaled K = 64 takes 205 us, with two stages (3 blocks) 235, with 256
-//    threads 272, with pieces of 1024 chunks and two stages 250.  Above K = 64
-//    four warps' maxima are too few for a threshold: K = 128 takes 496 us with
-//    256 threads and 2069 with 128.
+//    threads 272, with pieces of 1024 chunks 250.  Above K = 64 four warps'
+//    maxima are too few for a threshold: K = 128 takes 510 us with 256 threads
+//    and 2069 with 128.
 //  * No alternatives: pieces of 1024 chunks, two stages, 128 threads: 86 us
 //    scaled and 81 for 50k; one stage of 2048 and 256 threads 92 and 100.
 //  * Distillation: 256 threads, pieces of 2048 chunks, two stages: 207 us scaled

@@ -143,7 +143,8 @@ template <int R> __device__ __forceinline__ void sort_keys(unsigned long long (&
 // A warp's chunks whose largest logit passes, by their index in the piece, and
 // then their elements that pass, as many lanes a chunk as it has elements: few
 // chunks pass, and a warp that branched at each of them would run the elements'
-// code once for nearly every chunk (measured 1.6 times the whole kernel).
+// code once for nearly every chunk (4096 x 50000 bf16, K = 32: 223 instead of 178
+// us).
 struct Passing {
   unsigned short *list;                          // LIST of them
   int n = 0;
@@ -477,7 +478,7 @@ __device__ __noinline__ void select_row(const T *row, int V, int K, float thr, u
 
 template <typename T, int TH, bool ENT, bool TOP>
 __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(const ScoreArgs a) {
-  constexpr int EV = Elem<T>::EV, W = TH / 32;
+  constexpr int W = TH / 32;
   extern __shared__ __align__(128) unsigned char s_dyn[];
   // two of each, for rows in turn
   __shared__ Part s_part[2][W];
