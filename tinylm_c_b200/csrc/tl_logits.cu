@@ -148,7 +148,7 @@ int check_rows(int dtype, long long ld, int N, int V, const char *what) {
 
 // A gradient may take its logits' own place (the same rows), nothing between.
 int check_in_place(const void *dz, long long ldd, const LogitRows &z) {
-  if (dz == z.p && ldd == z.ld) return TL_OK;
+  if (dz == z.p && (ldd == z.ld || z.N == 1)) return TL_OK;
   const size_t es = dtype_size(z.dtype);
   const uintptr_t a = reinterpret_cast<uintptr_t>(dz), b = reinterpret_cast<uintptr_t>(z.p);
   const uintptr_t a1 = a + ((size_t)(z.N - 1) * ldd + z.V) * es, b1 = b + ((size_t)(z.N - 1) * z.ld + z.V) * es;

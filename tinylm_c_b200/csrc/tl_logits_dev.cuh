@@ -11,7 +11,8 @@
 // The blocks stay on the GPU and take rows in turn; while one row is worked on
 // the share of the next is on its way by a bulk copy into another stage of
 // shared memory, so the memory system is busy throughout.  A row is read from
-// memory once, however often a kernel goes over it.
+// memory once, however often a kernel goes over it, but for distilled rows of
+// several pieces (distill_kernel).
 #pragma once
 #include <cfloat>
 #include <cooperative_groups.h>
