@@ -803,6 +803,12 @@ def main():
               "e2e": {"value": round(tps, 2), "unit": "tokens/s", "h2d_bytes_per_step": 0, "d2h_bytes_per_step": 0}})
         return 0
 
+    no_ref = None
+    if not args.no_cpu_baseline:
+        import oracle
+        if not oracle.has_ref():               # a tree built without the reference's sources: no CPU figures
+            args.no_cpu_baseline = True
+            no_ref = {"unavailable": "oracle/_ref/libtlref.so not built (needs the reference sources at build time)"}
     rk = Run(rank, world, local)
     if args.gemm_engine:
         rk.ops.set_gemm_engine(args.gemm_engine)
@@ -835,6 +841,8 @@ def main():
             if rank == 0:
                 out["configs"] = configs
     if rank == 0:
+        if no_ref:
+            out["cpu_baseline"] = no_ref
         emit(out)
     rk.close()
     return 0
