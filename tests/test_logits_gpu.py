@@ -368,6 +368,20 @@ def test_distill_odd_teachers_and_students(cuda, dtype, V, tail):
     assert (dz[6:12] == 0).all() and (loss[6:12] == 0).all()
 
 
+@pytest.mark.parametrize("dtype,N,V,K", [("bf16", 4, 20010, 88), ("f16", 3, 963, 113), ("f32", 200, 9000, 60)])
+def test_distill_close_student(cuda, dtype, N, V, K):
+    """A loss of a few hundredths, a difference of terms of log V = 7 to 10 whose fp32 rounding alone is
+    2^-21 to 2^-22 each.  From fp32 sums whose terms' errors have independent signs (a few u of 2^-24
+    on sums of up to V terms) 16 u = 1e-6 is left for a row's loss."""
+    rng = np.random.default_rng(V)
+    z, _ = make(rng, N, V, dtype)
+    ids, vals = teacher(rng, z, K, 2.0, True)
+    L, _, _, _ = ref.distill(f64(z), ids, vals, 2.0, True, None, 1.0, dtype)
+    loss = run_distill(z, ids, vals, 2.0, True, None, 1.0, torch.empty_like(z))
+    assert 1e-3 < np.median(L) < 0.2
+    ref.close(loss.cpu(), L, 16 * ref.U, "loss")
+
+
 @pytest.mark.parametrize("tail", [False, True])
 def test_distill_whole_vocabulary(cuda, tail):
     """A teacher that names every token leaves no tail."""

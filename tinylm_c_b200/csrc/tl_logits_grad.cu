@@ -104,7 +104,8 @@ struct DistillArgs {
   const int *t_ids;
   const float *t_vals;
   int K;
-  float c, inv_t;
+  float c, inv_t;                    // log2(e) / temperature, 1 / temperature
+  double per_t;                      // 1 / temperature
   const float *weight;
   float scale;
   float *loss;
@@ -170,13 +171,16 @@ __device__ __forceinline__ void teach(const DistillArgs &a, const Chunks<T> &r, 
     tm = fmaxf(tm, l.t[k]);
   }
   if (!TAIL) tm = warp_max(tm);
-  float q[KL], all = 0.0f;
+  float q[KL];
+  double mass = 0.0;                             // 1 - sum q keeps what fp32 entries say of it
 #pragma unroll
   for (int k = 0; k < KL; k++) {
     q[k] = l.id[k] < 0 ? 0.0f : expf(TAIL ? l.t[k] : (l.t[k] - tm) * a.inv_t);
-    all += q[k];
+    mass += (double)q[k];
   }
-  all = warp_sum(all);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) mass += __shfl_xor_sync(FULL, mass, o);
+  const float all = (float)mass;
   const float inv = TAIL ? 1.0f : all == 0.0f ? 0.0f : 1.0f / all;
 #pragma unroll
   for (int k = 0; k < KL; k++) {
@@ -190,7 +194,7 @@ __device__ __forceinline__ void teach(const DistillArgs &a, const Chunks<T> &r, 
   if (lane == 0) {
     float Q = TAIL || all == 0.0f ? all : 1.0f;
     if (!(all < INFINITY)) Q = NAN;              // a NaN or +inf among the values
-    const float qr = TAIL ? 1.0f - Q : 0.0f;
+    const float qr = TAIL ? (Q == Q ? (float)(1.0 - mass) : Q) : 0.0f;
     sum[0] = Q;
     sum[1] = qr < TAIL_MIN ? 0.0f : qr;          // NaN stays
   }
@@ -242,27 +246,35 @@ struct RowLoss {
     m = warp_max(m);
     float sum = 0.0f;
     for (int j = lane; j < a.K; j += 32)
-      if (!(s.qv[j] < 0.0f)) sum += exp2_fast((s.z[j] - m) * a.c);
-    f = exp2_fast(bounded((p.m - m) * a.c));
+      if (!(s.qv[j] < 0.0f)) sum += exp2f((s.z[j] - m) * a.c);
+    f = exp2f(bounded((p.m - m) * a.c));
     all = fmaf(p.s, f, warp_sum(sum));
   }
+  // The row's loss, by one warp.  It is small where the student is close to its
+  // teacher, and a difference of terms as large as log V: these are added up in
+  // double from the fp32 sums, which are good to about 1e-7 (all in fp32, the
+  // rounding of log s alone, 5e-7, was 3e-5 of the loss at V = 20010,
+  // temperature 2).
   template <bool TAIL>
   __device__ __forceinline__ void write_loss(const DistillArgs &a, const Part &p, const Entries &s, int n, float w) const {
     const int lane = threadIdx.x & 31;
-    const float ls = logf(all);
-    float L = 0.0f;
+    // the row's three logarithms, a lane each
+    const double logs = log((double)(lane == 0 ? all : lane == 1 ? p.s : qr)), per = a.per_t;
+    const double ls = __shfl_sync(FULL, logs, 0), lrest = __shfl_sync(FULL, logs, 1), lqr = __shfl_sync(FULL, logs, 2);
+    double L = 0.0;
     for (int j = lane; j < a.K; j += 32) {
       const float qv = s.qv[j];
-      if (qv > 0.0f) L += qv * (logf(qv) - ((s.z[j] - m) * a.inv_t - ls));
+      if (qv > 0.0f) L += (double)qv * ((double)logf(qv) - (((double)s.z[j] - (double)m) * per - ls));
     }
-    L = warp_sum(L);
-    if (TAIL && qr > 0.0f) L += qr * (logf(qr) - (logf(p.s) + (p.m - m) * a.inv_t - ls));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(FULL, L, o);
+    if (TAIL && qr > 0.0f) L += (double)qr * (lqr - (lrest + ((double)p.m - (double)m) * per - ls));
     if (all == 0.0f) L = total > 0.0f ? INFINITY : 0.0f;       // a student that allows no token
     if (all != all || total != total) L = NAN;
-    L *= w;
+    L *= (double)w;
     if (lane == 0) {
-      if (a.loss) a.loss[n] = L;
-      if (a.loss64) a.loss64[n] = (double)L;
+      if (a.loss) a.loss[n] = (float)L;
+      if (a.loss64) a.loss64[n] = L;
     }
   }
   // The factor of e_v of the tokens not named; g = dL's factor.
@@ -609,7 +621,8 @@ int k_distill_topk(DeviceCtx *c, const LogitRows &z, const int *t_ids, const flo
                    void *dlogits, long long ldd) {
   TraceScope ts(c, "k_distill_topk");
   const RowPlan pl = plan_rows(c, z, 0, true);
-  const lg::DistillArgs a{pl.l, t_ids, t_vals, K, lg::LOG2E / temperature, 1.0f / temperature, weight, scale, loss,
+  const lg::DistillArgs a{pl.l, t_ids, t_vals, K, lg::LOG2E / temperature, 1.0f / temperature,
+                          1.0 / (double)temperature, weight, scale, loss,
                           loss64, dlogits, ldd, c->err_flag};
   if (z.dtype == TL_F32) return tail ? distill_typed<float, true>(c, pl, a) : distill_typed<float, false>(c, pl, a);
   if (z.dtype == TL_BF16)
