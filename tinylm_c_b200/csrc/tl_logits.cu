@@ -31,8 +31,9 @@ namespace tl {
 //    and 2069 with 128.
 //  * No alternatives: pieces of 1024 chunks, two stages, 128 threads: 86 us
 //    scaled and 81 for 50k; one stage of 2048 and 256 threads 92 and 100.
-//  * Distillation: 256 threads, pieces of 2048 chunks, two stages: 207 us scaled
-//    with a tail (with one stage 224) and 104 for 2048 x 50000 fp16 (123).  Rows
+//  * Distillation: 256 threads, pieces of 2048 chunks, two stages: 219 us scaled
+//    with a tail and 105 for 2048 x 50000 fp16 (two stages against one, before
+//    the loss was added up in double: 207 against 224 and 104 against 123).  Rows
 //    of six pieces or more, which come twice, three stages: so two blocks an SM,
 //    whose rows stay in L2 in between, 218 us for 2048 rows of 131k against 242.
 //  * Short rows, up to 256 chunks, have one computing warp, if its 32 maxima are
