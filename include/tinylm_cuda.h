@@ -235,7 +235,9 @@ int tl_model_step_zero1(void *handle, float *P, float *G, float *M_shard, float 
  * TL_VOCAB_MAX,
  * 1e-6 <= temperature <= 1e6.  With y = z/temperature:
  *   log p_v = y_v - log sum_u exp(y_u),   H = -sum_v p_v log p_v.
- * Sums, statistics and every float output are fp32 whatever the logits' type.
+ * Sums over the vocabulary, statistics and every float output are fp32 whatever
+ * the logits' type; what a distilled row's K entries give, and its loss, are
+ * worked out in double.
  * A logit of -inf is a token of probability 0.  A row of -inf only has
  * log p = -inf, H = 0 and no gradient; a type's lowest finite value is an
  * ordinary logit (a row of it is uniform).  A row holding a NaN or +inf has no

@@ -290,16 +290,16 @@ template <typename T> struct Piece {
 template <typename T> struct Pipe {
   uint4 *buf;                          // stage 0
   int stages, stage_chunks;
-  uint64_t *full;                      // a barrier a stage: a piece has arrived
   int *abort_flag;                     // a wait ran out: nothing is waited for or copied any more
   int *err;
   __device__ __forceinline__ uint4 *stage(int s) const { return buf + (size_t)s * stage_chunks; }
   // Piece p into stage s (`read` false: nothing is copied, the stage is full
-  // at once), by one thread.  The stage's earlier readers are done.  The
-  // tensor's first and last chunk, where it does not fill them, are written
-  // by the calling thread.
-  __device__ __forceinline__ void issue(const Rows<T> &t, int n, int piece, int s, bool read, uint64_t policy) const {
-    const uint32_t bar = tc::smem_u32(&full[s]);
+  // at once), by one thread; barrier `arrived` completes a phase when it is
+  // there.  The stage's earlier readers are done.  The tensor's first and last
+  // chunk, where it does not fill them, are written by the calling thread.
+  __device__ __forceinline__ void issue(const Rows<T> &t, int n, int piece, int s, uint64_t *arrived, bool read,
+                                        uint64_t policy) const {
+    const uint32_t bar = tc::smem_u32(arrived);
     if (*(volatile int *)abort_flag) return;
     int lo = 0, hi = 0;
     const uint4 *from = nullptr;
@@ -336,7 +336,7 @@ template <typename T> struct Pipe {
     tc::mbar_wait(tc::smem_u32(bar), parity, abort_flag, err, ERR_COPY);
   }
 };
-// Stage and phase of the k-th piece through a pipe.
+// Place and phase of the k-th use of a ring (stages, barriers).
 struct Turn {
   int s = 0;
   uint32_t phase = 0;

@@ -103,9 +103,9 @@ struct DistillArgs {
   Layout l;
   const int *t_ids;
   const float *t_vals;
-  int K;
-  float c, inv_t;                    // log2(e) / temperature, 1 / temperature
-  double per_t;                      // 1 / temperature
+  int K, tail;
+  float c;                           // log2(e) / temperature
+  double per;                        // 1 / temperature
   const float *weight;
   float scale;
   float *loss;
@@ -119,20 +119,44 @@ struct DistillArgs {
 // + q_r (log q_r - log p_r), p_r = sum of p over the others; Q = sum q + q_r.
 //   named v:  dL/dy_v = Q p_v - q_v
 //   others:   dL/dy_v = p_v (Q - q_r / p_r)
-// With a tail the named tokens are taken out of the row (set to -inf in shared
-// memory) before its statistics, so that p_r is summed and never 1 - sum p,
-// which loses all its digits for a confident student.  All others' gradients
-// are then one factor times e_v; the named tokens' are written over them at
-// the end.
+// Where the student is confident or close to its teacher these are small
+// differences: Q p_v - q_v of p and q near 1, 1 - sum q, log q - log p.  So the
+// K entries of a row are worked out in double by one warp, the teacher's side
+// (q, the tail) a row ahead, the student's (the named tokens' e relative to
+// their own largest logit) as the row arrives.  The named tokens are taken out of the row (set to -inf in shared
+// memory) before its statistics, so these are of the others alone, in fp32.
+// An error of theirs (about 1e-7) is then one factor 1 + delta of p_r, and
+// moves p_n = 1 - p_r by delta p_r p_n only; taken together in fp32 it would
+// move both by delta (in 1 of 10 cases of few rows the loss was then off by
+// more than 1e-5 of itself, up to all of it).  All others' gradients are one
+// factor times e_v; the named tokens' are written over them at the end.
 //
-// A row's entries in shared memory, K of each: the token (-1: padding), its q
-// and logit, and the mass of the token an entry stands for (-1 if it stands
-// for none: entries naming one token add up, the first of them stands for it).
+// A row's entries in shared memory, K of each in places that rows take in turn:
+// the token (-1: padding), its share of the teacher's mass before it is
+// normalised (entries naming one token add up, the first of them stands for it;
+// -1 for the others of them and for padding) and its e.
+constexpr int PLACES = 2;
 struct Entries {
+  static constexpr int BITS = 9;
+  double *q, *e;
   int *id;
-  float *q, *z, *qv;
-  __device__ __forceinline__ Entries(void *p, int K, int flip)
-      : id(static_cast<int *>(p) + flip * 4 * K), q(static_cast<float *>(p) + (flip * 4 + 1) * K), z(q + K), qv(z + K) {}
+  unsigned char *table;                          // of the warp that works them out, see teach()
+  static __host__ __device__ __forceinline__ int even(int K) { return (K + 1) & ~1; }
+  static __host__ __device__ __forceinline__ int bytes(int K) { return PLACES * even(K) * (2 * 8 + 4) + (1 << BITS); }
+  __device__ __forceinline__ Entries(void *p, int K, int place)
+      : q(static_cast<double *>(p) + place * even(K)), e(q + PLACES * even(K)),
+        id(reinterpret_cast<int *>(static_cast<double *>(p) + 2 * PLACES * even(K)) + place * even(K)),
+        table(reinterpret_cast<unsigned char *>(static_cast<double *>(p) + 2 * PLACES * even(K)) + PLACES * even(K) * 4) {}
+};
+// What else of a row's teacher, and of the student's side of its tokens.
+struct Taught {
+  double named, tail;                            // sum of q over the named tokens, q_r
+  double mass;                                   // sum of the entries' shares
+  double own;                                    // sum of share (log share - (z - m) / temperature)
+  double s;                                      // sum of e over the named tokens
+  float m;                                       // the named tokens' largest logit, what e is relative to
+  // q of an entry is its share times this
+  __device__ __forceinline__ double norm(bool tail) const { return tail || mass == 0.0 ? 1.0 : 1.0 / mass; }
 };
 constexpr int KL = TL_TOPK_MAX / 32;             // entries a lane
 
@@ -154,132 +178,182 @@ struct Loaded {
     }
   }
 };
-// The teacher's distribution from a row's loaded entries, by one warp: the
-// entries in shared memory, sum[0] the sum of q, sum[1] the tail.
-template <typename T, bool TAIL>
-__device__ __forceinline__ void teach(const DistillArgs &a, const Chunks<T> &r, Loaded &l, const Entries &to, float *sum) {
+// The teacher's distribution from a row's loaded entries, by one warp; `own` of
+// the result still lacks the student's logits.
+__device__ __forceinline__ Taught teach(const DistillArgs &a, Loaded &l, const Entries &to) {
   const int lane = threadIdx.x & 31;
-  float z[KL], tm = -FLT_MAX;
+  float tm = -FLT_MAX;
 #pragma unroll
   for (int k = 0; k < KL; k++) {
+    const int j = k * 32 + lane;
     if ((unsigned)l.id[k] >= (unsigned)a.l.V) {
       if (l.id[k] != -1) atomicExch(a.err, ERR_TOKEN);
       l.id[k] = -1;
       l.t[k] = -INFINITY;
     }
-    z[k] = l.id[k] >= 0 ? Elem<T>::to_f(r.row[l.id[k]]) : -INFINITY;
     tm = fmaxf(tm, l.t[k]);
+    if (j < a.K) to.id[j] = l.id[k];
   }
-  if (!TAIL) tm = warp_max(tm);
-  float q[KL];
-  double mass = 0.0;                             // 1 - sum q keeps what fp32 entries say of it
-#pragma unroll
-  for (int k = 0; k < KL; k++) {
-    q[k] = l.id[k] < 0 ? 0.0f : expf(TAIL ? l.t[k] : (l.t[k] - tm) * a.inv_t);
-    mass += (double)q[k];
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) mass += __shfl_xor_sync(FULL, mass, o);
-  const float all = (float)mass;
-  const float inv = TAIL ? 1.0f : all == 0.0f ? 0.0f : 1.0f / all;
-#pragma unroll
-  for (int k = 0; k < KL; k++) {
-    const int j = k * 32 + lane;
-    if (j < a.K) {
-      to.id[j] = l.id[k];
-      to.q[j] = to.qv[j] = q[k] * inv;
-      to.z[j] = z[k];
-    }
-  }
-  if (lane == 0) {
-    float Q = TAIL || all == 0.0f ? all : 1.0f;
-    if (!(all < INFINITY)) Q = NAN;              // a NaN or +inf among the values
-    const float qr = TAIL ? (Q == Q ? (float)(1.0 - mass) : Q) : 0.0f;
-    sum[0] = Q;
-    sum[1] = qr < TAIL_MIN ? 0.0f : qr;          // NaN stays
-  }
-  __syncwarp();
+  tm = warp_max(tm);
+  double mass = 0.0, own = 0.0;
 #pragma unroll
   for (int k = 0; k < KL; k++) {
     const int j = k * 32 + lane;
     if (k * 32 < a.K) {
-      bool again = false;
-      for (int i = 0; i < a.K; i++) again |= to.id[i] == l.id[k] && i != j;
-      if (l.id[k] < 0) {
-        if (j < a.K) to.qv[j] = -1.0f;
-      } else if (again) {
-        float qv = 0.0f;
-        bool first = true;
-        for (int i = 0; i < a.K; i++)
-          if (to.id[i] == l.id[k]) {
-            qv += to.q[i];
-            first = first && i >= j;
-          }
-        to.qv[j] = first ? qv : -1.0f;
+      const double u = a.tail ? (double)l.t[k] : ((double)l.t[k] - (double)tm) * a.per, x = exp(u);
+      if (j < a.K) to.q[j] = l.id[k] >= 0 ? x : -1.0;
+      if (l.id[k] >= 0) {
+        mass += x;
+        if (x > 0.0) own += x * u;               // its logarithm is known
       }
     }
   }
-}
-// The named tokens of a piece in shared memory set to -inf, by the warp that
-// loaded the entries.
-template <typename T> __device__ __forceinline__ void take_out(const Piece<T> &p, T *st, const Loaded &l) {
-  constexpr int EV = Elem<T>::EV;
+  __syncwarp();
+  // Whether the row names a token twice: the lanes compare theirs; where a lane
+  // has several, entries that fall into one place of a table are told apart by
+  // the one that stays there, the others try again.
+  unsigned open = 0;                             // a bit each of the lane's entries not told apart yet
+  bool twice = false;
+  if (a.K <= 32) {
+    twice = __popc(__match_any_sync(FULL, l.id[0])) > 1 && l.id[0] >= 0;
+  } else {
 #pragma unroll
-  for (int k = 0; k < KL; k++) {
-    const int at = l.id[k] + p.r.mis - p.c0 * EV;              // element of the piece
-    if (l.id[k] >= 0 && at >= 0 && at < p.cnt * EV) st[at] = Elem<T>::none();
+    for (int k = 0; k < KL; k++) open |= l.id[k] >= 0 ? 1u << k : 0;
+  }
+  auto place = [&](int k) { return &to.table[(unsigned)l.id[k] * 2654435769u >> (32 - Entries::BITS)]; };
+  while (__any_sync(FULL, open != 0)) {
+#pragma unroll
+    for (int k = 0; k < KL; k++)
+      if (open >> k & 1) *place(k) = (unsigned char)(k * 32 + lane);
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < KL; k++)
+      if (open >> k & 1) {
+        const int j = *place(k);
+        const bool mine = j == k * 32 + lane, same = !mine && to.id[j] == l.id[k];
+        twice |= same;
+        if (mine || same) open ^= 1u << k;
+      }
+    __syncwarp();
+  }
+  if (__any_sync(FULL, twice)) {
+    unsigned again = 0;                          // a bit each of the lane's entries whose token an earlier one names
+#pragma unroll 1
+    for (int k = 0; k * 32 < a.K; k++) {
+      const int j = k * 32 + lane, id = j < a.K ? to.id[j] : -1;
+      if (id < 0) continue;
+      double q = to.q[j];
+      for (int i = 0; i < a.K; i++)
+        if (to.id[i] == id) {
+          if (i < j) again |= 1u << k;
+          if (i > j) q += to.q[i];
+        }
+      if (!(again >> k & 1)) to.q[j] = q;        // read by no other lane: it stands first
+    }
+    __syncwarp();
+    own = 0.0;
+#pragma unroll 1
+    for (int j = lane, k = 0; j < a.K; j += 32, k++) {
+      const double x = to.q[j];
+      if (again >> k & 1) to.q[j] = -1.0;
+      else if (x > 0.0) own += x * log(x);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    mass += __shfl_xor_sync(FULL, mass, o);
+    own += __shfl_xor_sync(FULL, own, o);
+  }
+  double Q = a.tail || mass == 0.0 ? mass : 1.0;
+  if (!(mass < (double)INFINITY)) Q = (double)NAN;             // a NaN or +inf among the values
+  double qr = a.tail ? 1.0 - Q : 0.0;
+  if (qr < (double)TAIL_MIN) qr = 0.0;           // NaN stays
+  __syncwarp();
+  return Taught{Q, qr, mass, own, 0.0, -FLT_MAX};
+}
+// The tokens that a row's entries stand for (q not negative) and that lie in a
+// piece in shared memory: their logits go to e, and -inf to their
+// place in the piece.  By the warp that worked the entries out; m becomes the
+// lane's largest logit.
+template <typename T> __device__ __forceinline__ void take_out(const DistillArgs &a, const Piece<T> &p, T *st, const Entries &s, float &m) {
+  constexpr int EV = Elem<T>::EV;
+  for (int j = threadIdx.x & 31; j < a.K; j += 32) {
+    const int at = s.id[j] + p.r.mis - p.c0 * EV;              // element of the piece
+    if (!(s.q[j] < 0.0) && at >= 0 && at < p.cnt * EV) {
+      const float z = Elem<T>::to_f(st[at]);
+      s.e[j] = (double)z;
+      m = fmaxf(m, z);
+      st[at] = Elem<T>::none();
+    }
   }
   tc::fence_proxy_async();                       // a later copy into this stage comes after these writes
 }
-
-// What the gradient and the loss of a row go by, from its statistics p (with a
-// tail: of the tokens not named) and its entries; the same in every warp.
-struct RowLoss {
-  float m, all, f, total, qr;                    // e relative to p.m, times f, is relative to m; all: its sum
-  __device__ __forceinline__ RowLoss(const Part &p, const float *sum)
-      : m(p.m), all(p.s), f(1.0f), total(sum[0] + sum[1]), qr(sum[1]) {}
-  template <bool TAIL>
-  __device__ __forceinline__ void named(const DistillArgs &a, const Part &p, const Entries &s) {
-    if (!TAIL) return;
-    const int lane = threadIdx.x & 31;
-    for (int j = lane; j < a.K; j += 32) m = fmaxf(m, s.z[j]);
-    m = warp_max(m);
-    float sum = 0.0f;
-    for (int j = lane; j < a.K; j += 32)
-      if (!(s.qv[j] < 0.0f)) sum += exp2f((s.z[j] - m) * a.c);
-    f = exp2f(bounded((p.m - m) * a.c));
-    all = fmaf(p.s, f, warp_sum(sum));
+// The student's side of the row's tokens from their logits in e, m the lane's
+// largest of them, by that warp; lane 0 writes the result.
+__device__ __forceinline__ void look_at_student(const DistillArgs &a, const Entries &s, float m, Taught t, Taught *out) {
+  const int lane = threadIdx.x & 31;
+  t.m = warp_max(m);
+  double sum = 0.0, own = 0.0;
+#pragma unroll 2
+  for (int j = lane; j < a.K; j += 32) {
+    const double q = s.q[j];
+    if (q < 0.0) continue;
+    const double d = (s.e[j] - (double)t.m) * a.per, e = exp(d);
+    s.e[j] = e;
+    sum += e;
+    if (q > 0.0) own += q * d;
   }
-  // The row's loss, by one warp.  It is small where the student is close to its
-  // teacher, and a difference of terms as large as log V: these are added up in
-  // double from the fp32 sums, which are good to about 1e-7 (all in fp32, the
-  // rounding of log s alone, 5e-7, was 3e-5 of the loss at V = 20010,
-  // temperature 2).
-  template <bool TAIL>
-  __device__ __forceinline__ void write_loss(const DistillArgs &a, const Part &p, const Entries &s, int n, float w) const {
-    const int lane = threadIdx.x & 31;
-    // the row's three logarithms, a lane each
-    const double logs = log((double)(lane == 0 ? all : lane == 1 ? p.s : qr)), per = a.per_t;
-    const double ls = __shfl_sync(FULL, logs, 0), lrest = __shfl_sync(FULL, logs, 1), lqr = __shfl_sync(FULL, logs, 2);
-    double L = 0.0;
-    for (int j = lane; j < a.K; j += 32) {
-      const float qv = s.qv[j];
-      if (qv > 0.0f) L += (double)qv * ((double)logf(qv) - (((double)s.z[j] - (double)m) * per - ls));
-    }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(FULL, L, o);
-    if (TAIL && qr > 0.0f) L += (double)qr * (lqr - (lrest + ((double)p.m - (double)m) * per - ls));
-    if (all == 0.0f) L = total > 0.0f ? INFINITY : 0.0f;       // a student that allows no token
-    if (all != all || total != total) L = NAN;
+  for (int o = 16; o; o >>= 1) {
+    sum += __shfl_xor_sync(FULL, sum, o);
+    own += __shfl_xor_sync(FULL, own, o);
+  }
+  t.s = sum;
+  t.own -= own;
+  if (lane == 0) *out = t;
+  __syncwarp();
+}
+
+// What the gradient and the loss of a row go by, from the statistics p of the
+// tokens not named and its teacher; the same in every thread.
+struct RowLoss {
+  double fn, n, r, all;                          // n, r: the sums of e of the named and of the others, relative to one logit
+  __device__ __forceinline__ RowLoss(const DistillArgs &a, const Part &p, const Taught &t) {
+    const float m = fmaxf(p.m, t.m);
+    fn = (double)exp2f((t.m - m) * a.c);
+    n = t.s * fn;
+    r = (double)p.s * (double)exp2f((p.m - m) * a.c);
+    all = n + r;
+  }
+  // The row's loss, by one warp: a difference of terms as large as log V that
+  // is small where the student is close to its teacher, so in double throughout.
+  __device__ __forceinline__ static void write(const DistillArgs &a, const Part &p, const Taught &t, int n, float w) {
+    const int lane = threadIdx.x & 31;
+    const double m = fmax((double)p.m, (double)t.m), dn = ((double)t.m - m) * a.per, dr = ((double)p.m - m) * a.per;
+    // a lane each for what takes two exponentials and three logarithms
+    const double e = exp(lane == 0 ? dn : dr) * (lane == 0 ? t.s : (double)p.s);
+    const double all = __shfl_sync(FULL, e, 0) + __shfl_sync(FULL, e, 1);
+    const bool shares = !a.tail && t.mass != 0.0;
+    const double logs = log(lane == 0 ? all : lane == 1 ? (double)p.s : shares ? t.mass : t.tail);
+    const double lall = __shfl_sync(FULL, logs, 0), lrest = __shfl_sync(FULL, logs, 1), lq = __shfl_sync(FULL, logs, 2);
+    double L = shares ? t.own / t.mass - lq : t.own;
+    if (t.named > 0.0) L -= t.named * (dn - lall);
+    if (t.tail > 0.0) L += t.tail * (lq - (lrest + dr - lall));
+    const double total = t.named + t.tail;
+    if (all == 0.0) L = total > 0.0 ? (double)INFINITY : 0.0;  // a student that allows no token
+    if (all != all || total != total) L = (double)NAN;
     L *= (double)w;
     if (lane == 0) {
       if (a.loss) a.loss[n] = (float)L;
       if (a.loss64) a.loss64[n] = L;
     }
   }
-  // The factor of e_v of the tokens not named; g = dL's factor.
-  template <bool TAIL> __device__ __forceinline__ float factor(const Part &p, float g) const {
-    return all == 0.0f ? 0.0f : g * (total * f / all - (TAIL && qr > 0.0f && p.s > 0.0f ? qr / p.s : 0.0f));
+  // The factor of e_v of the tokens not named, g times
+  //   Q r / (all s) - q_r / s = (q_n r - q_r n) / (all s),
+  // the difference in double: near 0 for a student close to its teacher.
+  __device__ __forceinline__ float factor(const Part &p, const Taught &t, double g) const {
+    if (all == 0.0 || p.s == 0.0f) return 0.0f;
+    return (float)g * ((float)(t.named * r - t.tail * n) / (float)(all * (double)p.s));
   }
 };
 
@@ -331,22 +405,22 @@ template <typename T> struct Out {
     }
   }
   // The named tokens' gradients, those in chunks [c0, c0 + cnt).
-  __device__ __forceinline__ void named(const DistillArgs &a, const Entries &s, const RowLoss &l, float g, int c0, int cnt,
-                                        int t, int TH) const {
-    if (l.all == 0.0f) return;
-    for (int j = t; j < a.K; j += TH) {
-      const float q = s.qv[j];
-      if (q < 0.0f) continue;
+  __device__ __forceinline__ void named(const DistillArgs &a, const Entries &s, const Taught &t, const RowLoss &l, double g,
+                                        int c0, int cnt, int tid, int TH) const {
+    if (l.all == 0.0 || tid >= a.K) return;
+    const double f = (t.named + t.tail) * l.fn / l.all, norm = t.norm(a.tail);
+    for (int j = tid; j < a.K; j += TH) {
+      const double q = s.q[j] * norm;
+      if (q < 0.0) continue;
       const int id = s.id[j], at = (id + r.mis) / EV;
       if (at < c0 || at >= c0 + cnt) continue;
-      const float p = exp2_fast((s.z[j] - l.m) * a.c) / l.all;
-      o.row[id] = Elem<T>::from_f(g * (l.total * p - q));
+      o.row[id] = Elem<T>::from_f((float)(g * (s.e[j] * f - q)));
     }
   }
 };
 
 // Few rows, each split over the blocks of a cluster, a piece a block.
-template <typename T, int TH, bool TAIL>
+template <typename T, int TH>
 __global__ void __launch_bounds__(TH, min_blocks(TH)) distill_cluster_kernel(const DistillArgs a) {
   using TM = Team;
   constexpr int W = TH / 32;
@@ -354,20 +428,20 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) distill_cluster_kernel(con
   // two of each, for rows in turn: a barrier of the next row lies between a
   // row's last reads and the row after that's writes
   __shared__ Part s_part[2][W], s_from[2][MAX_CLUSTER];
-  __shared__ float s_sum[2][2];
+  __shared__ Taught s_teacher[2];
   __shared__ uint64_t s_full;
   __shared__ int s_abort;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int S = (int)TM::size(), rank = (int)TM::rank();
   const Rows<T> t(a.l);
   const int N = a.l.N, stride = (int)gridDim.x / S, first_row = (int)blockIdx.x / S;
-  const Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), 1, a.l.chunks, &s_full, &s_abort, a.err};
+  const Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), 1, a.l.chunks, &s_abort, a.err};
   auto counts = [&](int n) { return !a.weight || a.weight[n] != 0.0f; };
   if (tid == 0) {
     tc::mbar_init(tc::smem_u32(&s_full), 1);
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    pipe.issue(t, first_row, rank, 0, counts(first_row), l2_normal());
+    pipe.issue(t, first_row, rank, 0, &s_full, counts(first_row), l2_normal());
   }
   TM::sync();
   uint32_t phase = 0;
@@ -387,179 +461,240 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) distill_cluster_kernel(con
       }
       pipe.wait(&s_full, phase);
       TM::sync();
-      if (tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, next_counts, l2_normal());
+      if (tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, &s_full, next_counts, l2_normal());
       continue;
     }
-    Loaded l;
-    if (warp == 0) {
+    if (warp == 0) {                             // the tokens' logits from memory: another block may hold them
+      Loaded l;
       l.load(a, n);
-      teach<T, TAIL>(a, pc.r, l, s, s_sum[flip]);
+      const Taught of = teach(a, l, s);
+      float m = -FLT_MAX;
+      for (int j = lane; j < a.K; j += 32)
+        if (!(s.q[j] < 0.0)) {
+          const float z = Elem<T>::to_f(pc.r.row[s.id[j]]);
+          s.e[j] = (double)z;
+          m = fmaxf(m, z);
+        }
+      look_at_student(a, s, m, of, &s_teacher[flip]);
     }
     pipe.wait(&s_full, phase);
     if (t.ragged) pc.mask_ends(pipe.stage(0), [&](int i) { return i % TH == tid; });
-    if (TAIL) {
-      if (warp == 0) take_out(pc, reinterpret_cast<T *>(s_dyn), l);
-      __syncthreads();
+    if (warp == 0) {
+      for (int j = lane; j < a.K; j += 32) {
+        const int at = s.id[j] + pc.r.mis - pc.c0 * Elem<T>::EV;
+        if (s.id[j] >= 0 && at >= 0 && at < pc.cnt * Elem<T>::EV) reinterpret_cast<T *>(s_dyn)[at] = Elem<T>::none();
+      }
+      tc::fence_proxy_async();                   // a later copy into this stage comes after these writes
     }
+    __syncthreads();
     Running run;
     add_share<T, TH, false>(run, st, pc.cnt, a.c);
     Part p = run.warp<false>(a.c);
     if (lane == 0) s_part[flip][warp] = p;
     meet<false>(s_part[flip], s_from[flip], 0, a.c);
     p = join_all<false>(s_from[flip], S, a.c);
-    RowLoss row(p, s_sum[flip]);
-    row.named<TAIL>(a, p, s);
-    if (rank == 0 && warp == 0 && (a.loss || a.loss64)) row.write_loss<TAIL>(a, p, s, n, w);
-    const float g = w * a.scale * a.inv_t;
-    if (a.dz) out.template piece<TH, false>(st, pc.c0, pc.cnt, p, a.c, row.factor<TAIL>(p, g));
+    const Taught &teacher = s_teacher[flip];
+    const RowLoss row(a, p, teacher);
+    if (rank == 0 && warp == 0 && (a.loss || a.loss64)) RowLoss::write(a, p, teacher, n, w);
+    const double g = (double)w * (double)a.scale * a.per;
+    if (a.dz) out.template piece<TH, false>(st, pc.c0, pc.cnt, p, a.c, row.factor(p, teacher, g));
     __syncthreads();
-    if (tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, next_counts, l2_normal());
-    if (a.dz) out.named(a, s, row, g, pc.c0, pc.cnt, tid, TH);
+    if (tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, &s_full, next_counts, l2_normal());
+    if (a.dz) out.named(a, s, teacher, row, g, pc.c0, pc.cnt, tid, TH);
   }
   TM::sync();                                    // no block leaves while another may write to it
 }
 
 // Rows of one block each, in pieces one after another: TH threads compute, one
-// more warp keeps the pieces coming and one reads the teacher's entries a row
-// ahead and takes the named tokens out of the pieces.  A row of one piece is
+// more warp keeps the pieces coming and finishes rows (the named tokens'
+// gradients, the loss), and one works the teacher's entries out a row ahead and
+// takes the named tokens out of the pieces as they arrive.  A row of one piece is
 // kept in shared memory between the statistics and the gradient, a longer one
 // comes a second time, from L2 if the rows in flight fit there.
-template <typename T, int TH, bool TAIL>
+template <typename T, int TH>
 __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) distill_kernel(const DistillArgs a) {
   constexpr int W = TH / 32;
   extern __shared__ __align__(128) unsigned char s_dyn[];
-  __shared__ Part s_part[2][W];
-  __shared__ float s_sum[2][2], s_weight[2];
-  __shared__ uint64_t s_full[MAX_STAGES], s_ready[MAX_STAGES], s_free[MAX_STAGES], s_taught[2], s_spent[2];
+  __shared__ Part s_part[PLACES][W];
+  __shared__ Taught s_teacher[PLACES];
+  __shared__ float s_weight[PLACES];
+  // s_full, s_ready: of the pieces that come the first time, in a ring of their
+  // own (the teacher waits for these alone); s_late: of those that come again
+  __shared__ uint64_t s_full[MAX_STAGES], s_ready[MAX_STAGES], s_late[MAX_STAGES], s_free[MAX_STAGES];
+  // of a row: its weight is there, its entries are, the others' gradients are
+  // written, all of it is
+  __shared__ uint64_t s_taught[PLACES], s_seen[PLACES], s_spent[PLACES], s_over[PLACES];
   __shared__ int s_abort;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Rows<T> t(a.l);
   const int N = a.l.N, stride = (int)gridDim.x, first_row = (int)blockIdx.x, stages = a.l.stages, pieces = a.l.pieces;
   const int passes = a.dz && pieces > 1 ? 2 : 1;
   void *const entries = s_dyn + (size_t)stages * a.l.chunks * 16;
-  const Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), stages, a.l.chunks, s_full, &s_abort, a.err};
+  const Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), stages, a.l.chunks, &s_abort, a.err};
   if (tid == 0) {
     for (int i = 0; i < stages; i++) {
       tc::mbar_init(tc::smem_u32(&s_full[i]), 1);
       tc::mbar_init(tc::smem_u32(&s_ready[i]), 1);
+      tc::mbar_init(tc::smem_u32(&s_late[i]), 1);
       tc::mbar_init(tc::smem_u32(&s_free[i]), W);
     }
-    for (int i = 0; i < 2; i++) {
+    for (int i = 0; i < PLACES; i++) {
       tc::mbar_init(tc::smem_u32(&s_taught[i]), 1);
+      tc::mbar_init(tc::smem_u32(&s_seen[i]), 1);
       tc::mbar_init(tc::smem_u32(&s_spent[i]), W);
+      tc::mbar_init(tc::smem_u32(&s_over[i]), 1);
     }
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
-  if (warp == W) {                               // ---- the pieces
-    Turn put;
+  const int rows = (N - first_row + stride - 1) / stride;      // the block's
+  if (warp == W) {                               // ---- the pieces, and what is left of rows that are done
+    Turn put, early, late, over;                 // over: the place of the row that is finished next
     const uint64_t first = passes == 2 ? l2_again() : l2_normal(), last = l2_once();
-    int k = 0;
+    // a row is finished when the copies behind it are under way, as many as there are stages
+    const int total = passes * pieces, behind = total == 1 ? stages - 1 : 1, when = min(stages, total) - 1;
+    int issued = 0;
     float w = a.weight ? a.weight[first_row] : 1.0f;
-    for (int n = first_row; n < N; n += stride) {
-      const bool read = w != 0.0f;
-      if (a.weight && n + stride < N) w = a.weight[n + stride];
-      for (int i = 0; read && i < passes * pieces; i++, k++) {
-        if (k >= stages) pipe.wait(&s_free[put.s], put.phase ^ 1);
-        if (lane == 0) pipe.issue(t, n, i % pieces, put.s, true, i < pieces ? first : last);
+    for (int k = 0; k < rows + behind; k++) {
+      const int n = first_row + k * stride;
+      const bool read = k < rows && w != 0.0f;
+      if (a.weight && k + 1 < rows) w = a.weight[n + stride];
+      for (int i = 0; i == 0 || (read && i < total); i++) {
+        if (read) {
+          if (issued++ >= stages) pipe.wait(&s_free[put.s], put.phase ^ 1);
+          const bool again = i >= pieces;
+          if (lane == 0)
+            pipe.issue(t, n, again ? i - pieces : i, put.s, again ? &s_late[late.s] : &s_full[early.s], true,
+                       again ? last : first);
+          __syncwarp();
+          put.next(stages);
+          (again ? late : early).next(stages);
+        }
+        if (k < behind || i != (read ? when : 0)) continue;
+        const int done = n - behind * stride;
+        pipe.wait(&s_spent[over.s], over.phase);
+        const float wd = s_weight[over.s];
+        if (wd != 0.0f) {
+          const Part p = join_all<false>(s_part[over.s], W, a.c);
+          const Taught &teacher = s_teacher[over.s];
+          if (a.dz) {                            // the others' gradients are written
+            const Chunks<T> r = t.row(done);
+            Out<T>(a, r, done).named(a, Entries(entries, a.K, over.s), teacher, RowLoss(a, p, teacher),
+                                     (double)wd * (double)a.scale * a.per, 0, r.n, lane, 32);
+          }
+          if (a.loss || a.loss64) RowLoss::write(a, p, teacher, done, wd);
+        } else if (lane == 0) {
+          if (a.loss) a.loss[done] = 0.0f;
+          if (a.loss64) a.loss64[done] = 0.0;
+        }
         __syncwarp();
-        put.next(stages);
+        if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_over[over.s]));
+        over.next(PLACES);
       }
     }
     return;
   }
   if (warp == W + 1) {                           // ---- the teacher
-    Turn get;
-    Loaded next;
-    next.load(a, first_row);
-    float w_next = a.weight ? a.weight[first_row] : 1.0f;
-    int rows = 0;
-    for (int n = first_row; n < N; n += stride, rows++) {
-      const int flip = rows & 1;
-      Loaded l = next;
-      const float w = w_next;
-      if (n + stride < N) {
-        next.load(a, n + stride);
-        if (a.weight) w_next = a.weight[n + stride];
+    Turn get, early, at;                         // the stages, the barriers of pieces that come the first time, the places
+    Loaded l;                                    // the next row's entries
+    Taught of;                                   // the row's teacher, its student's part not yet there
+    l.load(a, first_row);
+    float w = 0.0f, w_next = a.weight ? a.weight[first_row] : 1.0f;
+    for (int k = 0; k <= rows; k++) {            // the block's k-th row
+      const int n = first_row + k * stride;
+      if (k >= 1) {                              // the row before, as it arrives
+        if (w != 0.0f) {
+          const Entries s(entries, a.K, at.s);
+          float m = -FLT_MAX;
+          for (int i = 0; i < pieces; i++) {
+            pipe.wait(&s_full[early.s], early.phase);
+            take_out(a, Piece<T>(t, n - stride, i), reinterpret_cast<T *>(pipe.stage(get.s)), s, m);
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_ready[early.s]));
+            early.next(stages);
+            get.next(stages);
+          }
+          // the second time the named tokens are written over anyway
+          for (int i = pieces; i < passes * pieces; i++) get.next(stages);
+          look_at_student(a, s, m, of, &s_teacher[at.s]);
+        }
+        if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_seen[at.s]));
+        at.next(PLACES);
       }
-      if (rows >= 2) pipe.wait(&s_spent[flip], ((rows >> 1) - 1) & 1);
-      if (w != 0.0f) teach<T, TAIL>(a, t.row(n), l, Entries(entries, a.K, flip), s_sum[flip]);
+      if (k == rows) break;
+      // this one's teacher, while the computing warps work on the row before
+      if (k >= PLACES) pipe.wait(&s_over[at.s], at.phase ^ 1);
+      w = w_next;
+      if (w != 0.0f) of = teach(a, l, Entries(entries, a.K, at.s));
       __syncwarp();
       if (lane == 0) {
-        s_weight[flip] = w;
-        tc::mbar_arrive(tc::smem_u32(&s_taught[flip]));
+        s_weight[at.s] = w;
+        tc::mbar_arrive(tc::smem_u32(&s_taught[at.s]));
       }
-      for (int i = 0; TAIL && w != 0.0f && i < passes * pieces; i++) {
-        pipe.wait(&s_full[get.s], get.phase);
-        // the second time the named tokens are written over anyway
-        if (i < pieces) take_out(Piece<T>(t, n, i), reinterpret_cast<T *>(pipe.stage(get.s)), l);
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_ready[get.s]));
-        get.next(stages);
+      if (k + 1 < rows) {
+        if (a.weight) w_next = a.weight[n + stride];
+        l.load(a, n + stride);
       }
     }
     return;
   }
   // ---- the computing warps
-  Turn turn;
+  Turn turn, early, late, at;
   auto arrived = [&] {
-    pipe.wait(&s_full[turn.s], turn.phase);
-    if (TAIL) pipe.wait(&s_ready[turn.s], turn.phase);
+    pipe.wait(&s_full[early.s], early.phase);
+    pipe.wait(&s_ready[early.s], early.phase);
+    early.next(stages);
+  };
+  auto arrived_again = [&] {
+    pipe.wait(&s_late[late.s], late.phase);
+    late.next(stages);
   };
   auto done = [&] {
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_free[turn.s]));
     turn.next(stages);
   };
-  int rows = 0;
-  for (int n = first_row; n < N; n += stride, rows++) {
-    const int flip = rows & 1;
-    const Entries s(entries, a.K, flip);
+  for (int k = 0; k < rows; k++) {
+    const int n = first_row + k * stride, place = at.s;
+    const uint32_t phase = at.phase;
     const Chunks<T> r = t.row(n);
     const Out<T> out(a, r, n);
-    pipe.wait(&s_taught[flip], (rows >> 1) & 1);
-    const float w = s_weight[flip];
+    pipe.wait(&s_taught[place], phase);
+    at.next(PLACES);
+    const float w = s_weight[place];
     if (w == 0.0f) {                             // a row that does not count is not read
       if (a.dz) out.zeros(0, r.n, tid, TH);
-      if (tid == 0) {
-        if (a.loss) a.loss[n] = 0.0f;
-        if (a.loss64) a.loss64[n] = 0.0;
-      }
     } else {
       Running run;
       for (int i = 0; i < pieces; i++) {
         arrived();
-        if (t.ragged) Piece<T>(t, n, i).mask_ends(pipe.stage(turn.s), [&](int k) { return k % TH == tid; });
+        if (t.ragged) Piece<T>(t, n, i).mask_ends(pipe.stage(turn.s), [&](int c) { return c % TH == tid; });
         add_share<T, TH, false>(run, tc::smem_u32(pipe.stage(turn.s)), max(0, min(r.n - i * t.per, t.per)), a.c);
         if (pieces > 1 || !a.dz) done();
       }
       Part p = run.warp<false>(a.c);
-      if (lane == 0) s_part[flip][warp] = p;
+      if (lane == 0) s_part[place][warp] = p;
+      pipe.wait(&s_seen[place], phase);
       bar_sync<TH>();
-      p = join_all<false>(s_part[flip], W, a.c);
-      RowLoss row(p, s_sum[flip]);
-      row.named<TAIL>(a, p, s);
-      const float g = w * a.scale * a.inv_t;
+      p = join_all<false>(s_part[place], W, a.c);
+      const Taught &teacher = s_teacher[place];
       if (a.dz) {
-        const float coef = row.factor<TAIL>(p, g);
+        const float coef = RowLoss(a, p, teacher).factor(p, teacher, (double)w * (double)a.scale * a.per);
         if (pieces == 1) {
           out.template piece<TH, false>(tc::smem_u32(pipe.stage(turn.s)), 0, r.n, p, a.c, coef);
           done();
         }
         for (int i = 0; pieces > 1 && i < pieces; i++) {
-          arrived();
+          arrived_again();
           out.template piece<TH, true>(tc::smem_u32(pipe.stage(turn.s)), i * t.per, max(0, min(r.n - i * t.per, t.per)),
                                        p, a.c, coef);
           done();
         }
-        bar_sync<TH>();
-        out.named(a, s, row, g, 0, r.n, tid, TH);
       }
-      if (warp == W - 1 && (a.loss || a.loss64)) row.write_loss<TAIL>(a, p, s, n, w);
     }
     __syncwarp();
-    if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_spent[flip]));
+    if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_spent[place]));
   }
 }
 
@@ -586,21 +721,22 @@ template <typename T> int grad_typed(DeviceCtx *c, const lg::GradArgs &a) {
   return launch_grad<T, 256>(c, nch, a);
 }
 
-template <typename T, int TH, bool TAIL> int launch_cluster(DeviceCtx *c, const RowPlan &pl, lg::DistillArgs a) {
+template <typename T, int TH> int launch_cluster(DeviceCtx *c, const RowPlan &pl, lg::DistillArgs a) {
   static Resident seen[kMaxDevices];
-  return launch_rows((const void *)lg::distill_cluster_kernel<T, TH, TAIL>, c, pl, 0, 32 * a.K, &seen[c->device], &a);
+  return launch_rows((const void *)lg::distill_cluster_kernel<T, TH>, c, pl, 0, lg::Entries::bytes(a.K), &seen[c->device],
+                     &a);
 }
-template <typename T, int TH, bool TAIL> int launch_distill(DeviceCtx *c, const RowPlan &pl, lg::DistillArgs a) {
+template <typename T, int TH> int launch_distill(DeviceCtx *c, const RowPlan &pl, lg::DistillArgs a) {
   static Resident seen[kMaxDevices];
-  return launch_rows((const void *)lg::distill_kernel<T, TH, TAIL>, c, pl, 64, 32 * a.K, &seen[c->device], &a);
+  return launch_rows((const void *)lg::distill_kernel<T, TH>, c, pl, 64, lg::Entries::bytes(a.K), &seen[c->device], &a);
 }
-template <typename T, bool TAIL> int distill_typed(DeviceCtx *c, const RowPlan &pl, const lg::DistillArgs &a) {
+template <typename T> int distill_typed(DeviceCtx *c, const RowPlan &pl, const lg::DistillArgs &a) {
   if (pl.blocks > 1) {
-    if (pl.threads == 128) return launch_cluster<T, 128, TAIL>(c, pl, a);
-    return pl.threads == 256 ? launch_cluster<T, 256, TAIL>(c, pl, a) : launch_cluster<T, 512, TAIL>(c, pl, a);
+    if (pl.threads == 128) return launch_cluster<T, 128>(c, pl, a);
+    return pl.threads == 256 ? launch_cluster<T, 256>(c, pl, a) : launch_cluster<T, 512>(c, pl, a);
   }
-  if (pl.threads == 32) return launch_distill<T, 32, TAIL>(c, pl, a);
-  return pl.threads == 128 ? launch_distill<T, 128, TAIL>(c, pl, a) : launch_distill<T, 256, TAIL>(c, pl, a);
+  if (pl.threads == 32) return launch_distill<T, 32>(c, pl, a);
+  return pl.threads == 128 ? launch_distill<T, 128>(c, pl, a) : launch_distill<T, 256>(c, pl, a);
 }
 
 }  // namespace
@@ -621,13 +757,11 @@ int k_distill_topk(DeviceCtx *c, const LogitRows &z, const int *t_ids, const flo
                    void *dlogits, long long ldd) {
   TraceScope ts(c, "k_distill_topk");
   const RowPlan pl = plan_rows(c, z, 0, true);
-  const lg::DistillArgs a{pl.l, t_ids, t_vals, K, lg::LOG2E / temperature, 1.0f / temperature,
-                          1.0 / (double)temperature, weight, scale, loss,
-                          loss64, dlogits, ldd, c->err_flag};
-  if (z.dtype == TL_F32) return tail ? distill_typed<float, true>(c, pl, a) : distill_typed<float, false>(c, pl, a);
-  if (z.dtype == TL_BF16)
-    return tail ? distill_typed<__nv_bfloat16, true>(c, pl, a) : distill_typed<__nv_bfloat16, false>(c, pl, a);
-  return tail ? distill_typed<__half, true>(c, pl, a) : distill_typed<__half, false>(c, pl, a);
+  const lg::DistillArgs a{pl.l, t_ids, t_vals, K, tail, lg::LOG2E / temperature, 1.0 / (double)temperature, weight, scale,
+                          loss, loss64, dlogits, ldd, c->err_flag};
+  if (z.dtype == TL_F32) return distill_typed<float>(c, pl, a);
+  if (z.dtype == TL_BF16) return distill_typed<__nv_bfloat16>(c, pl, a);
+  return distill_typed<__half>(c, pl, a);
 }
 
 }  // namespace tl

@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) score_cluster_kernel(const
   const Rows<T> t(a.l);
   const int N = a.l.N, stride = (int)gridDim.x / S, first_row = (int)blockIdx.x / S;
   unsigned long long *s_keys = reinterpret_cast<unsigned long long *>(s_dyn + (size_t)a.l.chunks * 16);
-  const Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), 1, a.l.chunks, &s_full, &s_abort, a.err};
+  const Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), 1, a.l.chunks, &s_abort, a.err};
   // full warps of this block, in every row: those whose 32 lanes all hold logits
   const int mine = max(0, min(min((a.l.V + EV - 1) / EV - rank * t.per, t.per), TH)) >> 5;
   const int g = a.j ? (a.K * mine + a.j * a.g_full - 1) / (a.j * a.g_full) : 0;
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) score_cluster_kernel(const
     tc::mbar_init(tc::smem_u32(&s_full), 1);
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    pipe.issue(t, first_row, rank, 0, true, l2_once());
+    pipe.issue(t, first_row, rank, 0, &s_full, true, l2_once());
     s_count[0] = s_count[1] = 0;
   }
   int id_next = reports && a.logp ? a.ids[first_row] : -1;
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) score_cluster_kernel(const
     meet<ENT>(s_part[flip], s_from[flip], g, a.c);
     const Part *parts = s_from[flip];
     const int ahead = n + stride;
-    if (!a.K && tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, true, l2_once());
+    if (!a.K && tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, &s_full, true, l2_once());
     unsigned found = 0;
     if (a.K) {                       // ---- the alternatives
       float thr = -INFINITY;         // too few maxima: every element passes
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) score_cluster_kernel(const
           found = *count;
         }
       }
-      if (tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, true, l2_once());
+      if (tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, &s_full, true, l2_once());
     }
     // ---- results: the first block's first warp, and all its warps where many
     // candidates are left to put in order
@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Rows<T> t(a.l);
   const int N = a.l.N, stride = (int)gridDim.x, first_row = (int)blockIdx.x, stages = a.l.stages, pieces = a.l.pieces;
-  const Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), stages, a.l.chunks, s_full, &s_abort, a.err};
+  const Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), stages, a.l.chunks, &s_abort, a.err};
   uint2 *s_keys = reinterpret_cast<uint2 *>(s_dyn + (size_t)stages * a.l.chunks * 16);     // [2][a.cap]
   if (tid == 0) {
     for (int i = 0; i < stages; i++) {
@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
     for (int n = first_row; n < N; n += stride)
       for (int i = 0; i < pieces; i++, k++) {
         if (k >= stages) pipe.wait(&s_free[put.s], put.phase ^ 1);
-        if (lane == 0) pipe.issue(t, n, i, put.s, true, l2_once());
+        if (lane == 0) pipe.issue(t, n, i, put.s, &s_full[put.s], true, l2_once());
         __syncwarp();
         put.next(stages);
       }
