@@ -266,7 +266,8 @@ int tl_token_logprobs(const void *logits, int dtype, long long ld, const int *id
 /* Gradient of sum_n dlogp[n] logp[n] + dentropy[n] entropy[n] in the logits,
  * written over dlogits (the logits' type, row stride ldd >= V):
  *   dz_v = (dlogp (1[v = id] - p_v) - dentropy p_v (log p_v + H)) / temperature
- * with stats and entropy of tl_token_logprobs at the same temperature.  dlogp
+ * with stats and entropy of tl_token_logprobs at the same temperature
+ * (|dentropy| / temperature up to 2^119, where fp32 ends).  dlogp
  * (with ids) or dentropy (with entropy) may be NULL.  dlogits may be logits
  * itself (ldd = ld); other overlap is TL_EINVAL.  A row to which nothing comes
  * back (dlogp and dentropy 0, or an id of -1) gets zeros and is not read. */

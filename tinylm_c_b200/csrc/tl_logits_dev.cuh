@@ -69,11 +69,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// max(x, -1e30), NaN kept: an exponent whose power is 0 anyway, made finite so
-// that power times exponent is 0 and not NaN.
-__device__ __forceinline__ float bounded(float x) {
+// max(x, LEAST), NaN kept: an exponent whose power is 0 anyway, made finite so
+// that power times exponent is 0 and not NaN.  -1e30 is below every difference
+// of logits that counts; where the exponent meets a factor of the caller's
+// first, -256 leaves that room (fp32 powers end at 2^-126).
+template <int LEAST = 0> __device__ __forceinline__ float bounded(float x) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(-1e30f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(LEAST ? (float)LEAST : -1e30f));
   return r;
 }
 // The warp's largest value (NaN only if all are).

@@ -60,7 +60,8 @@ __global__ void __launch_bounds__(256) token_logprobs_bwd_kernel(const GradArgs 
     if (!unread && c >= r.full0 && c < r.full1) x[i] = __ldcg(r.base + c);
     else if (!unread && c < r.n) x[i] = r.load_edge(c);
   }
-  // log2 p = (z - m) c - ls log2(e); the factor of p: -(a + b (log p + H))
+  // log2 p = (z - m) c - ls log2(e); the factor of p: -(a + b (log p + H)).  A
+  // token without probability has a finite factor up to |b| = 2^119.
   const float nl = -ls * LOG2E, fb = -gb * LN2, fa = -fmaf(gb, H, ga);
   const f32x2 nm2 = pack2(-m, -m), c2 = pack2(a.c, a.c), nl2 = pack2(nl, nl), fb2 = pack2(fb, fb), fa2 = pack2(fa, fa);
 #pragma unroll
@@ -76,7 +77,7 @@ __global__ void __launch_bounds__(256) token_logprobs_bwd_kernel(const GradArgs 
       float l0, l1;
       unpack2(l2, l0, l1);
       const f32x2 p2 = pack2(exp2_fast(l0), exp2_fast(l1));
-      const f32x2 k2 = ENT ? fma2(pack2(bounded(l0), bounded(l1)), fb2, fa2) : fa2;
+      const f32x2 k2 = ENT ? fma2(pack2(bounded<-256>(l0), bounded<-256>(l1)), fb2, fa2) : fa2;
       unpack2(mul2(p2, k2), f[e], f[e + 1]);
     }
     if ((unsigned)(id - v) < (unsigned)EV && id >= 0) {
