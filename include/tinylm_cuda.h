@@ -85,7 +85,10 @@ int tl_sync(void);
 int tl_set_host_buffers(int on);
 /* Wait for the stream, then report (and clear) the device error word that
  * bounded waits inside library kernels set when they give up: TL_ETIMEOUT if
- * any kernel since the last call returned early, else TL_OK. */
+ * any kernel since the last call returned early, else TL_OK.  (The results of
+ * such a call are not to be used.  TL_COPY_TIMEOUT_NS in the environment at
+ * tl_init shortens what the vocabulary-row kernels wait for their copies, two
+ * seconds otherwise; it is there to test this.) */
 int tl_device_status(void);
 
 /* Kernel tracing: when on, every library kernel launch is bracketed by CUDA

@@ -27,6 +27,7 @@ struct DeviceCtx {
   double *sumsq = nullptr;             // [1] scratch for tl_grad_norm
   float *scalars = nullptr;            // [4] scratch: norm, gscale
   int *err_flag = nullptr;             // device error word set by bounded waits
+  unsigned copy_wait_ns = 2000000000u; // how long the vocabulary-row kernels wait for a copy (TL_COPY_TIMEOUT_NS)
   float *gemm_ws = nullptr;            // split-K partial outputs
   size_t gemm_ws_floats = 0;
   unsigned *gemm_amax = nullptr;       // [8] operand max |x| (float bits) for the fp16-split GEMM

@@ -45,7 +45,7 @@ RowPlan plan_rows(const DeviceCtx *c, const LogitRows &z, int K, bool twice) {
   const int mis = one ? (int)(reinterpret_cast<uintptr_t>(z.p) & 15) / es : ev - 1;
   const int nch = (z.V + mis + ev - 1) / ev;
   constexpr int kPiece = 2048, kMostPerBlock = 6144;           // of a cluster: 96 KB in one stage
-  RowPlan p{256, 1, {z.p, z.ld, z.N, z.V, nch, 1, 1, 0, 0}};
+  RowPlan p{256, 1, {z.p, z.ld, z.N, z.V, nch, 1, 1, 0, 0, c->copy_wait_ns}};
   if (nch > kPiece && z.N <= c->num_sms) {
     p.blocks = 2;
     while (z.N * p.blocks * 2 <= c->num_sms && p.blocks < 8) p.blocks *= 2;

@@ -119,6 +119,16 @@ __device__ __forceinline__ uint4 lds(uint32_t a) {
 template <int TH> __device__ __forceinline__ void bar_sync() {
   asm volatile("bar.sync 1, %0;" ::"n"(TH) : "memory");
 }
+// The same, and whether any of the threads says so.
+template <int TH> __device__ __forceinline__ bool bar_any(bool x) {
+  uint32_t r;
+  asm volatile(
+      "{ .reg .pred p, q; setp.ne.u32 p, %1, 0; bar.red.or.pred q, 1, %2, p; selp.u32 %0, 1, 0, q; }"
+      : "=r"(r)
+      : "r"((uint32_t)x), "n"(TH)
+      : "memory");
+  return r != 0;
+}
 
 // ------------------------------------------------------------ element types
 template <typename T> struct Elem;
@@ -246,6 +256,7 @@ struct Layout {
   const void *z;
   long long ld;
   int N, V, per, pieces, stages, chunks, ragged;
+  unsigned wait_ns;                    // how long a wait lasts at most
 };
 template <typename T> struct Rows {
   const T *z;
@@ -289,20 +300,36 @@ template <typename T> struct Piece {
 };
 
 // The stages of a block and their barriers.
+//
+// Every wait ends: after `wait_ns` it sets the block's abort flag and the error
+// word, and from then on all waits that are not met at once fail and nothing is
+// copied any more.  A warp whose wait failed goes by nothing that the wait was
+// to protect: in the one-block kernels it leaves its loop without arriving
+// anywhere, so that the others' order holds until their own waits fail, and
+// the computing warps, which have a barrier without a time limit in common,
+// carry the failure to that barrier and leave together.  A cluster's blocks
+// meet whatever happened and run over the rows left, which are addressed by
+// what does not come from a copy.  Whoever issues copies drains them before it
+// leaves: shared memory that a copy is still to write is given up by no block.
 template <typename T> struct Pipe {
   uint4 *buf;                          // stage 0
   int stages, stage_chunks;
+  unsigned wait_ns;
   int *abort_flag;                     // a wait ran out: nothing is waited for or copied any more
   int *err;
+  __device__ __forceinline__ Pipe(void *buf_, const Layout &l, int stages_, int *abort_flag_, int *err_)
+      : buf(static_cast<uint4 *>(buf_)), stages(stages_), stage_chunks(l.chunks), wait_ns(l.wait_ns),
+        abort_flag(abort_flag_), err(err_) {}
   __device__ __forceinline__ uint4 *stage(int s) const { return buf + (size_t)s * stage_chunks; }
   // Piece p into stage s (`read` false: nothing is copied, the stage is full
   // at once), by one thread; barrier `arrived` completes a phase when it is
   // there.  The stage's earlier readers are done.  The tensor's first and last
   // chunk, where it does not fill them, are written by the calling thread.
-  __device__ __forceinline__ void issue(const Rows<T> &t, int n, int piece, int s, uint64_t *arrived, bool read,
+  // False after an expired wait.
+  __device__ __forceinline__ bool issue(const Rows<T> &t, int n, int piece, int s, uint64_t *arrived, bool read,
                                         uint64_t policy) const {
     const uint32_t bar = tc::smem_u32(arrived);
-    if (*(volatile int *)abort_flag) return;
+    if (*(volatile int *)abort_flag) return false;
     int lo = 0, hi = 0;
     const uint4 *from = nullptr;
     uint4 *st = stage(s);
@@ -329,13 +356,37 @@ template <typename T> struct Pipe {
               tc::smem_u32(st + lo)),
           "l"(__cvta_generic_to_global(from + lo)), "r"(bytes), "r"(bar), "l"(policy)
           : "memory");
+    return true;
   }
-  // Waits for a phase of a barrier, for two seconds at most.  After an expired
-  // wait the kernel runs on over what there is, its copies and waits over, and
-  // the error word says so: leaving would strand the other threads and blocks
-  // that meet this one.
-  __device__ __forceinline__ void wait(uint64_t *bar, uint32_t parity) const {
-    tc::mbar_wait(tc::smem_u32(bar), parity, abort_flag, err, ERR_COPY);
+  // Waits for a phase of a barrier; false where that did not come.
+  __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity) const {
+    const uint32_t at = tc::smem_u32(bar), suspend = min(wait_ns, tc::SUSPEND_NS);
+    const long long t0 = clock64();
+    while (!tc::mbar_try_wait(at, parity, suspend)) {
+      if (*(volatile int *)abort_flag) return false;
+      if (clock64() - t0 >= 2ll * wait_ns) {     // of a clock that ends below 2 GHz
+        *(volatile int *)abort_flag = 1;
+        atomicExch(err, ERR_COPY);
+        return false;
+      }
+    }
+    return true;
+  }
+  // The same for a whole warp, which goes on together.
+  __device__ __forceinline__ bool wait_all(uint64_t *bar, uint32_t parity) const {
+    return __all_sync(FULL, wait(bar, parity));
+  }
+  // Waits until the copies of the latest uses of a ring of barriers are there,
+  // `issued` uses in all, each for two seconds at most.
+  __device__ __forceinline__ void drain(uint64_t *ring, int size, int issued) const {
+    for (int u = max(0, issued - size); u < issued; u++) {
+      const long long t0 = clock64();
+      while (!tc::mbar_try_wait(tc::smem_u32(&ring[u % size]), (u / size) & 1))
+        if (clock64() - t0 > tc::WAIT_LIMIT_CYCLES) {
+          atomicExch(err, ERR_COPY);
+          break;
+        }
+    }
   }
 };
 // Place and phase of the k-th use of a ring (stages, barriers).

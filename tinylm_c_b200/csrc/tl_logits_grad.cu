@@ -198,15 +198,16 @@ __device__ __forceinline__ Taught teach(const DistillArgs &a, Loaded &l, const E
   tm = warp_max(tm);
   double mass = 0.0, own = 0.0;
 #pragma unroll
-  for (int k = 0; k < KL; k++) {
-    const int j = k * 32 + lane;
-    if (k * 32 < a.K) {
-      const double u = a.tail ? (double)l.t[k] : ((double)l.t[k] - (double)tm) * a.per, x = exp(u);
-      if (j < a.K) to.q[j] = l.id[k] >= 0 ? x : -1.0;
-      if (l.id[k] >= 0) {
-        mass += x;
-        if (x > 0.0) own += x * u;               // its logarithm is known
-      }
+  for (int k = 0; k < KL; k++)
+    if (k * 32 + lane < a.K) to.q[k * 32 + lane] = a.tail ? (double)l.t[k] : ((double)l.t[k] - (double)tm) * a.per;
+#pragma unroll 1                       // one copy of the code: unrolled, 16384 x 8192 fp32, K = 64 takes 230 instead of 218 us
+  for (int j = lane; j < a.K; j += 32) {
+    const double u = to.q[j], x = exp(u);
+    const bool is = to.id[j] >= 0;
+    to.q[j] = is ? x : -1.0;
+    if (is) {
+      mass += x;
+      if (x > 0.0) own += x * u;                 // its logarithm is known
     }
   }
   __syncwarp();
@@ -295,7 +296,7 @@ __device__ __forceinline__ void look_at_student(const DistillArgs &a, const Entr
   const int lane = threadIdx.x & 31;
   t.m = warp_max(m);
   double sum = 0.0, own = 0.0;
-#pragma unroll 2
+#pragma unroll 1
   for (int j = lane; j < a.K; j += 32) {
     const double q = s.q[j];
     if (q < 0.0) continue;
@@ -436,13 +437,14 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) distill_cluster_kernel(con
   const int S = (int)TM::size(), rank = (int)TM::rank();
   const Rows<T> t(a.l);
   const int N = a.l.N, stride = (int)gridDim.x / S, first_row = (int)blockIdx.x / S;
-  const Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), 1, a.l.chunks, &s_abort, a.err};
+  const Pipe<T> pipe(s_dyn, a.l, 1, &s_abort, a.err);
   auto counts = [&](int n) { return !a.weight || a.weight[n] != 0.0f; };
+  int issued = 0;                                // by thread 0
   if (tid == 0) {
     tc::mbar_init(tc::smem_u32(&s_full), 1);
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    pipe.issue(t, first_row, rank, 0, &s_full, counts(first_row), l2_normal());
+    issued += pipe.issue(t, first_row, rank, 0, &s_full, counts(first_row), l2_normal());
   }
   TM::sync();
   uint32_t phase = 0;
@@ -462,7 +464,7 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) distill_cluster_kernel(con
       }
       pipe.wait(&s_full, phase);
       TM::sync();
-      if (tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, &s_full, next_counts, l2_normal());
+      if (tid == 0 && ahead < N) issued += pipe.issue(t, ahead, rank, 0, &s_full, next_counts, l2_normal());
       continue;
     }
     if (warp == 0) {                             // the tokens' logits from memory: another block may hold them
@@ -500,9 +502,10 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) distill_cluster_kernel(con
     const double g = (double)w * (double)a.scale * a.per;
     if (a.dz) out.template piece<TH, false>(st, pc.c0, pc.cnt, p, a.c, row.factor(p, teacher, g));
     __syncthreads();
-    if (tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, &s_full, next_counts, l2_normal());
+    if (tid == 0 && ahead < N) issued += pipe.issue(t, ahead, rank, 0, &s_full, next_counts, l2_normal());
     if (a.dz) out.named(a, s, teacher, row, g, pc.c0, pc.cnt, tid, TH);
   }
+  if (tid == 0) pipe.drain(&s_full, 1, issued);
   TM::sync();                                    // no block leaves while another may write to it
 }
 
@@ -531,7 +534,7 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) distill_kernel(c
   const int N = a.l.N, stride = (int)gridDim.x, first_row = (int)blockIdx.x, stages = a.l.stages, pieces = a.l.pieces;
   const int passes = a.dz && pieces > 1 ? 2 : 1;
   void *const entries = s_dyn + (size_t)stages * a.l.chunks * 16;
-  const Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), stages, a.l.chunks, &s_abort, a.err};
+  const Pipe<T> pipe(s_dyn, a.l, stages, &s_abort, a.err);
   if (tid == 0) {
     for (int i = 0; i < stages; i++) {
       tc::mbar_init(tc::smem_u32(&s_full[i]), 1);
@@ -555,7 +558,7 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) distill_kernel(c
     const uint64_t first = passes == 2 ? l2_again() : l2_normal(), last = l2_once();
     // a row is finished when the copies behind it are under way, as many as there are stages
     const int total = passes * pieces, behind = total == 1 ? stages - 1 : 1, when = min(stages, total) - 1;
-    int issued = 0;
+    int issued = 0, early_issued = 0, late_issued = 0;
     float w = a.weight ? a.weight[first_row] : 1.0f;
     for (int k = 0; k < rows + behind; k++) {
       const int n = first_row + k * stride;
@@ -563,18 +566,18 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) distill_kernel(c
       if (a.weight && k + 1 < rows) w = a.weight[n + stride];
       for (int i = 0; i == 0 || (read && i < total); i++) {
         if (read) {
-          if (issued++ >= stages) pipe.wait(&s_free[put.s], put.phase ^ 1);
+          if (issued++ >= stages && !pipe.wait_all(&s_free[put.s], put.phase ^ 1)) goto out;
           const bool again = i >= pieces;
-          if (lane == 0)
-            pipe.issue(t, n, again ? i - pieces : i, put.s, again ? &s_late[late.s] : &s_full[early.s], true,
-                       again ? last : first);
-          __syncwarp();
+          const bool ok = lane != 0 || pipe.issue(t, n, again ? i - pieces : i, put.s,
+                                                  again ? &s_late[late.s] : &s_full[early.s], true, again ? last : first);
+          if (!__all_sync(FULL, ok)) goto out;
           put.next(stages);
           (again ? late : early).next(stages);
+          (again ? late_issued : early_issued)++;
         }
         if (k < behind || i != (read ? when : 0)) continue;
         const int done = n - behind * stride;
-        pipe.wait(&s_spent[over.s], over.phase);
+        if (!pipe.wait_all(&s_spent[over.s], over.phase)) goto out;
         const float wd = s_weight[over.s];
         if (wd != 0.0f) {
           const Part p = join_all<false>(s_part[over.s], W, a.c);
@@ -594,6 +597,11 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) distill_kernel(c
         over.next(PLACES);
       }
     }
+  out:
+    if (lane == 0) {
+      pipe.drain(s_full, stages, early_issued);
+      pipe.drain(s_late, stages, late_issued);
+    }
     return;
   }
   if (warp == W + 1) {                           // ---- the teacher
@@ -609,7 +617,7 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) distill_kernel(c
           const Entries s(entries, a.K, at.s);
           float m = -FLT_MAX;
           for (int i = 0; i < pieces; i++) {
-            pipe.wait(&s_full[early.s], early.phase);
+            if (!pipe.wait_all(&s_full[early.s], early.phase)) return;
             take_out(a, Piece<T>(t, n - stride, i), reinterpret_cast<T *>(pipe.stage(get.s)), s, m);
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_ready[early.s]));
@@ -625,7 +633,7 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) distill_kernel(c
       }
       if (k == rows) break;
       // this one's teacher, while the computing warps work on the row before
-      if (k >= PLACES) pipe.wait(&s_over[at.s], at.phase ^ 1);
+      if (k >= PLACES && !pipe.wait_all(&s_over[at.s], at.phase ^ 1)) return;
       w = w_next;
       if (w != 0.0f) of = teach(a, l, Entries(entries, a.K, at.s));
       __syncwarp();
@@ -642,60 +650,56 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) distill_kernel(c
   }
   // ---- the computing warps
   Turn turn, early, late, at;
-  auto arrived = [&] {
-    pipe.wait(&s_full[early.s], early.phase);
-    pipe.wait(&s_ready[early.s], early.phase);
-    early.next(stages);
-  };
-  auto arrived_again = [&] {
-    pipe.wait(&s_late[late.s], late.phase);
-    late.next(stages);
-  };
-  auto done = [&] {
+  auto done = [&](bool ok) {
     __syncwarp();
-    if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_free[turn.s]));
+    if (lane == 0 && ok) tc::mbar_arrive(tc::smem_u32(&s_free[turn.s]));
     turn.next(stages);
   };
+  bool ok = true;                                // of each lane; what it leaves undone only its own warp and the barrier see
   for (int k = 0; k < rows; k++) {
     const int n = first_row + k * stride, place = at.s;
     const uint32_t phase = at.phase;
     const Chunks<T> r = t.row(n);
     const Out<T> out(a, r, n);
-    pipe.wait(&s_taught[place], phase);
+    ok &= pipe.wait(&s_taught[place], phase);
     at.next(PLACES);
-    const float w = s_weight[place];
-    if (w == 0.0f) {                             // a row that does not count is not read
-      if (a.dz) out.zeros(0, r.n, tid, TH);
-    } else {
+    const float w = __all_sync(FULL, ok) ? s_weight[place] : 0.0f;
+    Part p = no_part();
+    if (w != 0.0f) {
       Running run;
       for (int i = 0; i < pieces; i++) {
-        arrived();
+        ok &= pipe.wait(&s_full[early.s], early.phase);
+        ok &= pipe.wait(&s_ready[early.s], early.phase);
+        early.next(stages);
         if (t.ragged) Piece<T>(t, n, i).mask_ends(pipe.stage(turn.s), [&](int c) { return c % TH == tid; });
         add_share<T, TH, false>(run, tc::smem_u32(pipe.stage(turn.s)), max(0, min(r.n - i * t.per, t.per)), a.c);
-        if (pieces > 1 || !a.dz) done();
+        if (pieces > 1 || !a.dz) done(ok);
       }
-      Part p = run.warp<false>(a.c);
+      p = run.warp<false>(a.c);
       if (lane == 0) s_part[place][warp] = p;
-      pipe.wait(&s_seen[place], phase);
-      bar_sync<TH>();
+      ok &= pipe.wait(&s_seen[place], phase);
+    }
+    if (bar_any<TH>(!ok)) return;                // else w is the same in all warps
+    if (w == 0.0f) {                             // a row that does not count is not read
+      if (a.dz) out.zeros(0, r.n, tid, TH);
+    } else if (a.dz) {
       p = join_all<false>(s_part[place], W, a.c);
       const Taught &teacher = s_teacher[place];
-      if (a.dz) {
-        const float coef = RowLoss(a, p, teacher).factor(p, teacher, (double)w * (double)a.scale * a.per);
-        if (pieces == 1) {
-          out.template piece<TH, false>(tc::smem_u32(pipe.stage(turn.s)), 0, r.n, p, a.c, coef);
-          done();
-        }
-        for (int i = 0; pieces > 1 && i < pieces; i++) {
-          arrived_again();
-          out.template piece<TH, true>(tc::smem_u32(pipe.stage(turn.s)), i * t.per, max(0, min(r.n - i * t.per, t.per)),
-                                       p, a.c, coef);
-          done();
-        }
+      const float coef = RowLoss(a, p, teacher).factor(p, teacher, (double)w * (double)a.scale * a.per);
+      if (pieces == 1) {
+        out.template piece<TH, false>(tc::smem_u32(pipe.stage(turn.s)), 0, r.n, p, a.c, coef);
+        done(true);
+      }
+      for (int i = 0; pieces > 1 && i < pieces; i++) {
+        ok &= pipe.wait(&s_late[late.s], late.phase);
+        late.next(stages);
+        out.template piece<TH, true>(tc::smem_u32(pipe.stage(turn.s)), i * t.per, max(0, min(r.n - i * t.per, t.per)), p,
+                                     a.c, coef);
+        done(ok);
       }
     }
     __syncwarp();
-    if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_spent[place]));
+    if (lane == 0 && ok) tc::mbar_arrive(tc::smem_u32(&s_spent[place]));
   }
 }
 

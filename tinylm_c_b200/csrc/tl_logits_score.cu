@@ -203,16 +203,17 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) score_cluster_kernel(const
   const Rows<T> t(a.l);
   const int N = a.l.N, stride = (int)gridDim.x / S, first_row = (int)blockIdx.x / S;
   unsigned long long *s_keys = reinterpret_cast<unsigned long long *>(s_dyn + (size_t)a.l.chunks * 16);
-  const Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), 1, a.l.chunks, &s_abort, a.err};
+  const Pipe<T> pipe(s_dyn, a.l, 1, &s_abort, a.err);
   // full warps of this block, in every row: those whose 32 lanes all hold logits
   const int mine = max(0, min(min((a.l.V + EV - 1) / EV - rank * t.per, t.per), TH)) >> 5;
   const int g = a.j ? (a.K * mine + a.j * a.g_full - 1) / (a.j * a.g_full) : 0;
   const bool reports = rank == 0 && tid == 0;    // the thread that writes a row's scalars
+  int issued = 0;                                // by thread 0
   if (tid == 0) {
     tc::mbar_init(tc::smem_u32(&s_full), 1);
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    pipe.issue(t, first_row, rank, 0, &s_full, true, l2_once());
+    issued += pipe.issue(t, first_row, rank, 0, &s_full, true, l2_once());
     s_count[0] = s_count[1] = 0;
   }
   int id_next = reports && a.logp ? a.ids[first_row] : -1;
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) score_cluster_kernel(const
     meet<ENT>(s_part[flip], s_from[flip], g, a.c);
     const Part *parts = s_from[flip];
     const int ahead = n + stride;
-    if (!a.K && tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, &s_full, true, l2_once());
+    if (!a.K && tid == 0 && ahead < N) issued += pipe.issue(t, ahead, rank, 0, &s_full, true, l2_once());
     unsigned found = 0;
     if (a.K) {                       // ---- the alternatives
       float thr = -INFINITY;         // too few maxima: every element passes
@@ -280,7 +281,7 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) score_cluster_kernel(const
           found = *count;
         }
       }
-      if (tid == 0 && ahead < N) pipe.issue(t, ahead, rank, 0, &s_full, true, l2_once());
+      if (tid == 0 && ahead < N) issued += pipe.issue(t, ahead, rank, 0, &s_full, true, l2_once());
     }
     // ---- results: the first block's first warp, and all its warps where many
     // candidates are left to put in order
@@ -334,6 +335,7 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) score_cluster_kernel(const
       }
     }
   }
+  if (tid == 0) pipe.drain(&s_full, 1, issued);
   TM::sync();                // the first block's memory stays until all have read it
 }
 
@@ -445,8 +447,10 @@ __device__ __noinline__ void select_row(const T *row, int V, int K, float thr, u
     Elem<T>::unpack(chunk(c), f);
 #pragma unroll
     for (int e = 0; e < EV; e++)
-      if (f[e] > -INFINITY && order_of(f[e]) >= hi)
-        keys[atomicAdd(s_count, 1u)] = make_uint2(__float_as_uint(f[e]), (unsigned)(r.first(c) + e));
+      if (f[e] > -INFINITY && order_of(f[e]) >= hi) {
+        const unsigned at = atomicAdd(s_count, 1u);            // below `above`, as long as nobody writes to the row meanwhile
+        if (at < (unsigned)cap) keys[at] = make_uint2(__float_as_uint(f[e]), (unsigned)(r.first(c) + e));
+      }
   }
   int have = above;
   for (int c0 = 0; have < K && c0 < r.n; c0 += TH) {
@@ -472,7 +476,7 @@ __device__ __noinline__ void select_row(const T *row, int V, int K, float thr, u
     have += sum[0];
   }
   bar_sync<TH>();
-  if (tid == 0) *s_count = few ? above : K;
+  if (tid == 0) *s_count = few ? min(above, cap) : K;
   bar_sync<TH>();
 }
 
@@ -490,7 +494,7 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Rows<T> t(a.l);
   const int N = a.l.N, stride = (int)gridDim.x, first_row = (int)blockIdx.x, stages = a.l.stages, pieces = a.l.pieces;
-  const Pipe<T> pipe{reinterpret_cast<uint4 *>(s_dyn), stages, a.l.chunks, &s_abort, a.err};
+  const Pipe<T> pipe(s_dyn, a.l, stages, &s_abort, a.err);
   uint2 *s_keys = reinterpret_cast<uint2 *>(s_dyn + (size_t)stages * a.l.chunks * 16);     // [2][a.cap]
   if (tid == 0) {
     for (int i = 0; i < stages; i++) {
@@ -511,11 +515,13 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
     int k = 0;
     for (int n = first_row; n < N; n += stride)
       for (int i = 0; i < pieces; i++, k++) {
-        if (k >= stages) pipe.wait(&s_free[put.s], put.phase ^ 1);
-        if (lane == 0) pipe.issue(t, n, i, put.s, &s_full[put.s], true, l2_once());
-        __syncwarp();
+        if (k >= stages && !pipe.wait_all(&s_free[put.s], put.phase ^ 1)) goto out;
+        const bool ok = lane != 0 || pipe.issue(t, n, i, put.s, &s_full[put.s], true, l2_once());
+        if (!__all_sync(FULL, ok)) goto out;
         put.next(stages);
       }
+  out:
+    if (lane == 0) pipe.drain(s_full, stages, k);
     return;
   }
   if (warp == W + 1) {               // ---- the results
@@ -529,7 +535,7 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
         else if (id != -1) atomicExch(a.err, ERR_TOKEN);
         if (n + stride < N) id = a.ids[n + stride];
       }
-      pipe.wait(&s_done[flip], phase);
+      if (!pipe.wait_all(&s_done[flip], phase)) return;
       const Part p = join_all<ENT>(s_part[flip], W, a.c);
       const float ls = logf(p.s);    // -inf where nothing is left, NaN for a row without a distribution
       const bool bad = !(p.s >= 0.0f);
@@ -546,7 +552,7 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
         }
       }
       if (TOP) {
-        const int found = bad ? 0 : (int)s_count[flip];
+        const int found = bad ? 0 : min((int)__shfl_sync(FULL, s_count[flip], 0), a.cap);
         const float thr = s_thr[flip];
         uint2 *keys = s_keys + flip * a.cap;
         int *to_id = a.top_ids + (size_t)n * a.K;
@@ -616,7 +622,8 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
   for (int n = first_row; n < N; n += stride, count_rows++) {
     const int flip = count_rows & 1;
     // this row's places in shared memory: the results' warp has taken the row before last from them
-    if (count_rows >= 2) pipe.wait(&s_taken[flip], ((count_rows >> 1) - 1) & 1);
+    const bool mine = count_rows < 2 || pipe.wait_all(&s_taken[flip], ((count_rows >> 1) - 1) & 1);
+    bool ok = mine;                  // of each lane
     const Chunks<T> r = t.row(n);
     uint2 *keys = s_keys + flip * a.cap;
     Running run;
@@ -640,12 +647,16 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
       const uint32_t st = tc::smem_u32(pipe.stage(turn.s));
       bool equal = false;
       auto flush = [&] {
+        if (!mine) {                 // the row's places may still be another's
+          pass.n = 0;
+          return;
+        }
         pass.elements<T>(reinterpret_cast<const T *>(pipe.stage(turn.s)), thr, equal, [&](float f, int v) {
           const unsigned at = atomicAdd(&s_count[flip], 1u);
           if (at < (unsigned)a.cap) keys[at] = make_uint2(__float_as_uint(f), (unsigned)(r.first(c0) + v));
         });
       };
-      pipe.wait(&s_full[turn.s], turn.phase);
+      ok &= pipe.wait(&s_full[turn.s], turn.phase);
       if (t.ragged) Piece<T>(t, n, i).mask_ends(pipe.stage(turn.s), [&](int k) { return k % TH == tid; });
       if (!TOP) {
         add_share<T, TH, ENT>(run, st, cnt, a.c);
@@ -683,15 +694,16 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
       }
       if (TOP) flush();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s_free[turn.s]));
+      if (lane == 0 && ok) tc::mbar_arrive(tc::smem_u32(&s_free[turn.s]));
       turn.next(stages);
     }
+    if (!TOP && !__all_sync(FULL, ok)) return;   // no barrier is left that the others wait at
     Part p = run.warp<ENT>(a.c);
-    if (lane == 0) s_part[flip][warp] = p;
+    if (lane == 0 && mine) s_part[flip][warp] = p;
     if (TOP) {
       if (a.j && pieces > 1) thr = fmaxf(thr, threshold());
-      if (tid == 0) s_thr[flip] = thr;
-      bar_sync<TH>();
+      if (tid == 0 && mine) s_thr[flip] = thr;
+      if (bar_any<TH>(!ok)) return;  // else the results' warp leaves s_count alone until this row is done
       if (s_count[flip] > (unsigned)a.cap) {
         p = join_all<false>(s_part[flip], W, a.c);
         if (p.s >= 0.0f)             // a row without a distribution has no alternatives

@@ -77,6 +77,10 @@ TL_API int tl_init(int device) {
   TL_TRY_CUDA(cudaMalloc(&c.gemm_ws, sizeof(float) * kGemmWorkspaceFloats));
   c.gemm_ws_floats = kGemmWorkspaceFloats;
   TL_TRY_CUDA(cudaMalloc(&c.gemm_amax, sizeof(unsigned) * 8));
+  if (const char *e = getenv("TL_COPY_TIMEOUT_NS")) {
+    const long long ns = atoll(e);
+    if (ns >= 0 && ns < (long long)c.copy_wait_ns) c.copy_wait_ns = (unsigned)ns;
+  }
   TL_TRY_CUDA(cudaDeviceSynchronize());
   c.ready = true;
   return TL_OK;
