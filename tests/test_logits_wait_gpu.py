@@ -59,6 +59,38 @@ print("ended", seen[_lib.TL_OK], seen[_lib.TL_ETIMEOUT])
 """
 
 
+TOKEN = """
+import torch
+from tinylm_c_b200 import _lib, ops
+ops.init(0)
+N, V, K = 3000, 300, 4
+z = torch.randn(N, V, device="cuda")
+v, t = torch.topk(z, K, dim=1)
+v, t, L = v.contiguous(), t.int().contiguous(), torch.empty(N, device="cuda")
+ids, a, stats = torch.full((N,), V, dtype=torch.int32, device="cuda"), torch.ones(N, device="cuda"), torch.ones(N, 2, device="cuda")
+for _ in range(20):
+    ops.distill_topk(z, t, v, N, V, K, L, torch.empty_like(z))
+torch.cuda.synchronize()
+for call in (lambda: ops.token_logprobs_bwd(torch.empty_like(z), z, ids, N, V, stats, a),
+             lambda: ops.token_logprobs(z, ids, N, V, a), lambda: ops.distill_topk(z, t + V, v, N, V, K, L)):
+    call()
+status = _lib.lib().tl_device_status
+print("status", status(), status())
+ops.token_logprobs_bwd(torch.empty_like(z), z, ids, N, V, stats, a)
+print(status())
+"""
+
+
+def test_a_bad_token_does_not_hide_an_expired_wait(cuda):
+    """The status after a wait that ran out is that, whatever a later call found in its ids."""
+    from tinylm_c_b200 import _lib
+    env = dict(os.environ, TL_COPY_TIMEOUT_NS="0")
+    r = subprocess.run([sys.executable, "-c", TOKEN], cwd=ROOT, capture_output=True, text=True, timeout=300, env=env)
+    assert r.returncode == 0, r.stderr[-2000:]
+    got = [int(x) for x in r.stdout.split("status")[1].split()]
+    assert got == [_lib.TL_ETIMEOUT, _lib.TL_OK, _lib.TL_EINVAL]
+
+
 @pytest.mark.parametrize("limit_ns", [2000000000, 100000, 10000, 3000, 1000, 300, 0])
 def test_waits_that_run_out(cuda, limit_ns):
     env = dict(os.environ, TL_COPY_TIMEOUT_NS=str(limit_ns))

@@ -35,6 +35,9 @@ constexpr int MAX_WARPS = 16, MAX_STAGES = 4;
 constexpr int min_blocks(int TH) { return 1024 / TH; }
 constexpr int ERR_COPY = 90;                       // error word: a bulk copy did not arrive in time
 constexpr int ERR_TOKEN = 100;                     // a token id outside [0, V)
+// The error word keeps an expired wait, whose results are lost: a token that is
+// taken as none does not replace it.
+__device__ __forceinline__ void report_token(int *err) { atomicCAS(err, 0, ERR_TOKEN); }
 
 // ------------------------------------------------------------- arithmetic
 // Two fp32 operations in one instruction (sm_100's packed pairs), each

@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(256) token_logprobs_bwd_kernel(const GradArgs 
   const int c0 = seg * (TPR * CPT) + t;
   int id = a.dlogp ? a.ids[n] : -1;
   if (id != -1 && (unsigned)id >= (unsigned)a.V) {
-    if (c0 == 0) atomicExch(a.err, ERR_TOKEN);
+    if (c0 == 0) report_token(a.err);
     id = -1;
   }
   const float m = a.stats[2 * n], ls = a.stats[2 * n + 1];
@@ -188,7 +188,7 @@ __device__ __forceinline__ Taught teach(const DistillArgs &a, Loaded &l, const E
   for (int k = 0; k < KL; k++) {
     const int j = k * 32 + lane;
     if ((unsigned)l.id[k] >= (unsigned)a.l.V) {
-      if (l.id[k] != -1) atomicExch(a.err, ERR_TOKEN);
+      if (l.id[k] != -1) report_token(a.err);
       l.id[k] = -1;
       l.t[k] = -INFINITY;
     }

@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(TH, min_blocks(TH)) score_cluster_kernel(const
       if (id >= 0 && id < t.V) {
         z_id = Elem<T>::to_f(sh.r.row[id]);
       } else {
-        if (id != -1) atomicExch(a.err, ERR_TOKEN);
+        if (id != -1) report_token(a.err);
         id = -1;
       }
       if (n + stride < N) id_next = a.ids[n + stride];
@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
       const int given = id;
       if (lane == 0 && a.logp) {
         if (id >= 0 && id < t.V) z_id = Elem<T>::to_f(t.z[(size_t)n * t.ld + id]);
-        else if (id != -1) atomicExch(a.err, ERR_TOKEN);
+        else if (id != -1) report_token(a.err);
         if (n + stride < N) id = a.ids[n + stride];
       }
       if (!pipe.wait_all(&s_done[flip], phase)) return;

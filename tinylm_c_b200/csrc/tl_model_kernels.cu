@@ -39,7 +39,7 @@ __global__ void embed_fwd_kernel(const float *__restrict__ emb, const int *__res
   if (n >= N) return;
   int t = tok[n];
   if (t < 0 || t >= V) {  // out-of-range token: record and use row 0
-    if (threadIdx.x == 0) atomicExch(err, 100);
+    if (threadIdx.x == 0) atomicCAS(err, 0, 100);
     t = 0;
   }
   const float *src = emb + (size_t)t * D;
