@@ -503,23 +503,34 @@ TL_API int tl_model_score(void *h, const float *P, const int *tok, const int *tg
   return score_batch(c, *m, P, tok, tgt, B, temperature, logp, entropy, K, top_ids, top_logp);
 }
 
+// What tl_model_distill and tl_model_distill_step refuse, before anything is written.
+static int check_distill(DeviceCtx *c, const Model &m, const float *P, const int *tok, const int *t_ids,
+                         const float *t_vals, int K, const float *weight, int B, float temperature, int tail,
+                         const float *loss_dev) {
+  if (c->device != m.device) return set_error(TL_EINVAL, "model belongs to device %d", m.device);
+  TRY(check_batch(m, B));
+  TRY(check_temperature(temperature));
+  TRY(check_topk(K, m.V));
+  if (m.V > TL_VOCAB_MAX) return set_error(TL_EINVAL, "V = %d above %d", m.V, TL_VOCAB_MAX);
+  if (K < 1) return set_error(TL_EINVAL, "K = 0: a teacher names at least one token");
+  if (tail != 0 && tail != 1) return set_error(TL_EINVAL, "tail %d is neither 0 nor 1", tail);
+  TRY(check_ptr_here(c, P, "P", 4));
+  TRY(check_ptr_here(c, tok, "tok", 4));
+  TRY(check_ptr_here(c, t_ids, "t_ids", 4));
+  TRY(check_ptr_here(c, t_vals, "t_vals", 4));
+  if (weight) TRY(check_ptr_here(c, weight, "weight", 4));
+  if (loss_dev) TRY(check_ptr_here(c, loss_dev, "loss_dev", 4));
+  return TL_OK;
+}
+
 TL_API int tl_model_distill(void *h, const float *P, float *G, const int *tok, const int *t_ids, const float *t_vals,
                             int K, const float *weight, int B, float temperature, int tail, float *loss_dev) {
   Model *m = static_cast<Model *>(h);
   if (!m) return set_error(TL_EINVAL, "NULL model");
   TL_REQUIRE_CTX(c);
-  if (c->device != m->device) return set_error(TL_EINVAL, "model belongs to device %d", m->device);
-  int rc;
-  if ((rc = check_batch(*m, B)) || (rc = check_temperature(temperature)) || (rc = check_topk(K, m->V))) return rc;
-  if (m->V > TL_VOCAB_MAX) return set_error(TL_EINVAL, "V = %d above %d", m->V, TL_VOCAB_MAX);
-  if (K < 1) return set_error(TL_EINVAL, "K = 0: a teacher names at least one token");
-  if (tail != 0 && tail != 1) return set_error(TL_EINVAL, "tail %d is neither 0 nor 1", tail);
+  TRY(check_distill(c, *m, P, tok, t_ids, t_vals, K, weight, B, temperature, tail, loss_dev));
   if (!G && !loss_dev) return set_error(TL_EINVAL, "no output asked for");
-  if ((rc = check_ptr_here(c, P, "P", 4)) || (rc = check_ptr_here(c, tok, "tok", 4)) ||
-      (rc = check_ptr_here(c, t_ids, "t_ids", 4)) || (rc = check_ptr_here(c, t_vals, "t_vals", 4)) ||
-      (G && (rc = check_ptr_here(c, G, "G", 4))) || (weight && (rc = check_ptr_here(c, weight, "weight", 4))) ||
-      (loss_dev && (rc = check_ptr_here(c, loss_dev, "loss_dev", 4))))
-    return rc;
+  if (G) TRY(check_ptr_here(c, G, "G", 4));
   return distill_batch(c, *m, P, G, tok, t_ids, t_vals, K, weight, B, temperature, tail, loss_dev);
 }
 
@@ -530,15 +541,15 @@ TL_API int tl_model_distill_step(void *h, float *P, float *G, float *M, float *V
   if (!m) return set_error(TL_EINVAL, "NULL model");
   TL_REQUIRE_CTX(c);
   if (t < 1) return set_error(TL_EINVAL, "step t must be >= 1 (got %d)", t);
-  int rc;
-  if ((rc = check_ptr_here(c, G, "G", 4)) || (rc = check_ptr_here(c, M, "M", 4)) || (rc = check_ptr_here(c, V, "V", 4)) ||
-      (norm_dev && (rc = check_ptr_here(c, norm_dev, "norm_dev", 4))))
-    return rc;
-  if (c->device != m->device) return set_error(TL_EINVAL, "model belongs to device %d", m->device);
+  TRY(check_distill(c, *m, P, tok, t_ids, t_vals, K, weight, B, temperature, tail, loss_dev));
+  TRY(check_ptr_here(c, G, "G", 4));
+  TRY(check_ptr_here(c, M, "M", 4));
+  TRY(check_ptr_here(c, V, "V", 4));
+  if (norm_dev) TRY(check_ptr_here(c, norm_dev, "norm_dev", 4));
   TL_TRY_CUDA(cudaMemsetAsync(G, 0, sizeof(float) * m->np, c->stream));
-  if ((rc = tl_model_distill(h, P, G, tok, t_ids, t_vals, K, weight, B, temperature, tail, loss_dev))) return rc;
+  TRY(distill_batch(c, *m, P, G, tok, t_ids, t_vals, K, weight, B, temperature, tail, loss_dev));
   float *gscale = c->scalars + 1;
-  if ((rc = launch_sumsq(c, G, m->np, c->sumsq, norm_dev, gscale, max_norm))) return rc;
+  TRY(launch_sumsq(c, G, m->np, c->sumsq, norm_dev, gscale, max_norm));
   return launch_adamw(c, P, G, M, V, m->np, lr, 0.9f, 0.95f, 0.1f, t, 1.0f, gscale);
 }
 
