@@ -19,6 +19,13 @@ def load_golden(name):
         return {k: z[k] for k in z.files}
 
 
+@pytest.fixture(autouse=True)
+def seeded():
+    """torch's generators start from the same seed in every test (the CUDA one is seeded from the clock otherwise)."""
+    import torch
+    torch.manual_seed(0)
+
+
 @pytest.fixture(scope="session")
 def golden():
     return load_golden

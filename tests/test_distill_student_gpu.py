@@ -1,4 +1,5 @@
-"""Distillation of the device model: what a refused step leaves as it was."""
+"""Distillation of the device model: its gradient against differences along it
+whose step error is taken out, and what a refused step leaves as it was."""
 import numpy as np
 import pytest
 import torch
@@ -21,6 +22,35 @@ def setting(cuda, B=2, K=16, tau=2.0):
     ids, lp = torch.empty(n, K, dtype=torch.int32, device=cuda), torch.empty(n, K, device=cuda)
     m.score(Pt, tok, None, B, None, K=K, top_ids=ids, top_logp=lp, temperature=tau)
     return m, P, tok, ids, lp, w, dict(K=K, B=B, weight=w, temperature=tau)
+
+
+@pytest.mark.parametrize("tail", [False, True])
+def test_gradient_against_differences(cuda, tail):
+    """f(P + h g) - f(P - h g) over 2 h |g|^2 is 1 + c h^2 + O(h^4) for the gradient g.  A step that
+    changes the loss by 1 % has c h^2 of 2 % at such weights, which the quotients of h and h / 2 take
+    out: (4 q(h/2) - q(h)) / 3 is off by O(h^4), a fourth of a percent of that 2 % or less where the
+    quotients' own distance from 1 falls by about 4; and by the losses' rounding, 2^-24 of a loss over
+    a change of 1 % of it, 2^-24 / 0.01 each, taken 16 / 3 and 4 / 3 times."""
+    m, P, tok, ids, lp, w, kw = setting(cuda)
+    G, loss = torch.zeros_like(P), torch.zeros(1, device=cuda)
+    m.distill(P, G, tok, ids, lp, tail=tail, loss_out=loss, **kw)
+    g2 = float(G.double().square().sum())
+
+    def quotient(h):
+        out = []
+        for x in (P + h * G, P - h * G):
+            m.distill(x, None, tok, ids, lp, tail=tail, loss_out=loss, **kw)
+            out.append(loss.item())
+        return (out[0] - out[1]) / (2 * h * g2)
+
+    h = 0.01 * loss.item() / g2
+    a, b = quotient(h), quotient(h / 2)
+    assert abs(a - 1) < 0.05                      # the step is small enough for the two terms to say it
+    # the model's products carry its gradients to 1e-4, the losses' rounding 8 * 2^-24 / 0.01, the step's
+    # fourth power a twentieth of its square's effect at most
+    tol = 1e-4 + 8 * 2.0 ** -24 / 0.01 + abs(a - 1) / 20
+    assert abs((4 * b - a) / 3 - 1) <= tol, (a, b)
+    m.close()
 
 
 def test_refused_steps_leave_the_gradient(cuda):
