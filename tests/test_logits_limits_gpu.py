@@ -49,3 +49,29 @@ def test_entropy_gradient_of_large_upstream_values(cuda, tau, b):
         tol = tol + 2.0 ** -126 * 128 * np.abs(up.astype(np.float64))[:, None] / tau
         ref.close(f64(dz), want, tol, f"dlogits {N} x {V} {dtype}")
     assert _lib.lib().tl_device_status() == _lib.TL_OK
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_sums_of_the_longest_rows(cuda, dtype):
+    """Rows of equal logits behind 2048 larger ones, 2^18 in all, more rows than SMs: every thread's terms
+    round the same way, so a sum shows how many it adds one after another.  The logarithm of a row's sum
+    is off by the sum's bound and its own rounding, the entropy by its bound."""
+    N, V, first = 300, 1 << 18, 2048
+    below = torch.linspace(0.01, 3.0, N, device="cuda").to(DT[dtype])
+    z = (-below)[:, None].expand(N, V).contiguous()
+    z[:, :first] = 0.0
+    logp, H, stats = torch.empty(N, device="cuda"), torch.empty(N, device="cuda"), torch.empty(N, 2, device="cuda")
+    ids = torch.arange(N, device="cuda", dtype=torch.int32) * 811 + first
+    ops.token_logprobs(z, ids, N, V, logp, entropy=H, stats=stats)
+    d = f64(below)
+    total = first + (V - first) * np.exp(-d)
+    ls = np.log(total)
+    ref.close(f64(stats[:, 1]), ls, ref.a_bound(V) + 2 * ref.U * ls, "log of the sum")
+    ref.close(f64(logp), -d - ls, ref.logp_bound(-d - ls, V), "logp")
+    ref.close(f64(H), ls + (V - first) * np.exp(-d) * d / total, ref.entropy_bound(V), "entropy")
+    # a loss is -log p of one named token
+    K, one = 1, torch.zeros(N, 1, device="cuda")
+    loss, dz = torch.empty(N, device="cuda"), torch.empty_like(z)
+    ops.distill_topk(z, ids[:, None].contiguous(), one, N, V, K, loss, dz)
+    ref.close(f64(loss), d + ls, ref.a_bound(V) + 2 * ref.U * (d + ls), "loss")
+    assert _lib.lib().tl_device_status() == _lib.TL_OK

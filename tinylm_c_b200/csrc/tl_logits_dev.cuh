@@ -469,9 +469,12 @@ template <typename T, int TH, typename F> __device__ __forceinline__ void for_ch
 }
 
 // This thread's running statistics of a row: m the largest logit so far, s and
-// t relative to it.
+// t relative to it, of the piece at hand (s2, t2) and of those before (s, t).
+// A piece adds at most 64 values to a sum one after another, so a long row's
+// rounding stays that of 64 and its pieces' additions (one sum for the whole
+// row: 1024 at 262144 logits).
 struct Running {
-  float m = -FLT_MAX, top = -INFINITY;
+  float m = -FLT_MAX, top = -INFINITY, s = 0.0f, t = 0.0f;
   f32x2 s2 = 0, t2 = 0;
   // Adds C chunks; the largest of their logits.
   template <typename T, bool ENT, int C> __device__ __forceinline__ float add(const uint4 (&x)[C], float c) {
@@ -483,8 +486,12 @@ struct Running {
     if (b > m) {                       // the sums move to the new reference
       const float d = bounded((m - b) * c), f = exp2_fast(d);
       const f32x2 f2 = pack2(f, f);
-      if (ENT) t2 = mul2(f2, fma2(s2, pack2(d, d), t2));
+      if (ENT) {
+        t2 = mul2(f2, fma2(s2, pack2(d, d), t2));
+        t = f * fmaf(s, d, t);
+      }
       s2 = mul2(s2, f2);
+      s *= f;
       m = b;
     }
     const f32x2 nm = pack2(-m, -m), cc = pack2(c, c);
@@ -503,19 +510,25 @@ struct Running {
     }
     return b;
   }
-  // The warp's part.
+  // A piece ends.
+  template <bool ENT> __device__ __forceinline__ void fold() {
+    float a, b;
+    unpack2(s2, a, b);
+    s += a + b;
+    s2 = 0;
+    if (ENT) {
+      unpack2(t2, a, b);
+      t += a + b;
+      t2 = 0;
+    }
+  }
+  // The warp's part, all pieces folded.
   template <bool ENT> __device__ __forceinline__ Part warp(float c) const {
     Part p = no_part();
     p.m = warp_max(m);
     const float d = bounded((m - p.m) * c), f = exp2_fast(d);
-    float a, b;
-    unpack2(s2, a, b);
-    const float s = a + b;
     p.s = warp_sum(s * f);
-    if (ENT) {
-      unpack2(t2, a, b);
-      p.t = warp_sum(f * fmaf(s, d, a + b));
-    }
+    if (ENT) p.t = warp_sum(f * fmaf(s, d, t));
     return p;
   }
 };
@@ -523,6 +536,7 @@ template <typename T, int TH, bool ENT>
 __device__ __forceinline__ void add_share(Running &run, uint32_t st, int cnt, float c) {
   for_chunks<T, TH>(st, cnt, [&](const uint4 (&x)[4], int) { run.add<T, ENT>(x, c); },
                  [&](const uint4 (&x)[1], int) { run.add<T, ENT>(x, c); });
+  run.fold<ENT>();
 }
 
 // The blocks of a row: `sync` is a barrier of all their threads.

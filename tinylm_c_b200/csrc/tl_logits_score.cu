@@ -691,6 +691,7 @@ __global__ void __launch_bounds__(TH + 64, min_blocks(TH + 64)) score_kernel(con
           pass.add(run.add<T, ENT>(x, a.c) > thr, k);
           if (pass.n > LIST - 4 * 32) flush();
         });
+        run.fold<ENT>();
       }
       if (TOP) flush();
       __syncwarp();
