@@ -272,8 +272,9 @@ int tl_token_logprobs(const void *logits, int dtype, long long ld, const int *id
  * with stats and entropy of tl_token_logprobs at the same temperature
  * (|dentropy| / temperature up to 2^119, where fp32 ends).  dlogp
  * (with ids) or dentropy (with entropy) may be NULL.  dlogits may be logits
- * itself (ldd = ld); other overlap is TL_EINVAL.  A row to which nothing comes
- * back (dlogp and dentropy 0, or an id of -1) gets zeros and is not read. */
+ * itself (ldd = ld), or between its rows (ldd = ld >= 2 V); rows that share
+ * elements otherwise, or seem to at other strides, are TL_EINVAL.  A row to
+ * which nothing comes back (dlogp and dentropy 0, or an id of -1) gets zeros and is not read. */
 int tl_token_logprobs_bwd(void *dlogits, long long ldd, const void *logits, int dtype, long long ld, const int *ids,
                           int N, int V, float temperature, const float *stats, const float *entropy,
                           const float *dlogp, const float *dentropy);

@@ -75,3 +75,50 @@ def test_sums_of_the_longest_rows(cuda, dtype):
     ops.distill_topk(z, ids[:, None].contiguous(), one, N, V, K, loss, dz)
     ref.close(f64(loss), d + ls, ref.a_bound(V) + 2 * ref.U * (d + ls), "loss")
     assert _lib.lib().tl_device_status() == _lib.TL_OK
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("N,V,gap", [(5, 100, 0), (4, 1001, 3), (400, 3001, 0), (200, 20011, 1)])
+def test_gradient_between_the_rows(cuda, dtype, N, V, gap):
+    """Logits and their gradient as the halves of one buffer's rows, in both orders: the same bits as
+    with the gradient in other memory (sums go by where in 16 bytes a row starts, so in the same places
+    there), the logits and what lies between left as they were."""
+    z = logits(V, N, V, dtype)
+    ids = torch.arange(N, device="cuda", dtype=torch.int32) % V
+    v, t = torch.topk(z.float(), 7, dim=1)
+    v, t = v.contiguous(), t.int().contiguous()
+    H, stats = scored(z, 1.0)
+    a, loss = torch.ones(N, device="cuda"), torch.empty(N, device="cuda")
+    for flip in (False, True):
+        both, other = (torch.full((N, 2 * V + gap), 77.0, dtype=DT[dtype], device="cuda") for _ in range(2))
+        at = [slice(0, V), slice(V + gap, 2 * V + gap)]
+        zi, di, own = both[:, at[flip]], both[:, at[not flip]], other[:, at[not flip]]
+        zi.copy_(z)
+        keep = both.clone()
+        for run in (lambda d: ops.token_logprobs_bwd(d, zi, ids, N, V, stats, a, entropy=H, dentropy=a),
+                    lambda d: ops.distill_topk(zi, t, v, N, V, 7, loss, d)):
+            run(own)
+            run(di)
+            assert torch.equal(di, own) and torch.equal(zi, z)
+        di.fill_(77.0)
+        assert torch.equal(both, keep)
+    assert _lib.lib().tl_device_status() == _lib.TL_OK
+
+
+def test_gradient_rows_that_share_elements(cuda):
+    """Refused: one element shared with the next row on either side, rows apart at another stride."""
+    V = 64
+    flat = torch.zeros(4000, device="cuda")
+    ids, out, stats = torch.zeros(4, dtype=torch.int32, device="cuda"), torch.empty(4, device="cuda"), torch.zeros(4, 2, device="cuda")
+
+    def rows(start, ld):
+        return torch.as_strided(flat, (4, V), (ld, 1), start)
+
+    for z, d in ((rows(0, 2 * V), rows(V - 1, 2 * V)), (rows(0, 2 * V), rows(V + 1, 2 * V)), (rows(V + 1, 2 * V), rows(0, 2 * V)),
+                 (rows(0, 2 * V), rows(V, 2 * V + 1)), (rows(0, 2 * V - 1), rows(V, 2 * V - 1))):
+        with pytest.raises(_lib.TLError) as e:
+            ops.token_logprobs_bwd(d, z, ids, 4, V, stats, out)
+        assert e.value.code == _lib.TL_EINVAL
+        with pytest.raises(_lib.TLError):
+            ops.distill_topk(z, ids, out, 4, V, 1, out, d)
+    ops.token_logprobs_bwd(rows(V, 2 * V), rows(0, 2 * V), ids, 4, V, stats, out)

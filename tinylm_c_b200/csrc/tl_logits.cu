@@ -147,15 +147,20 @@ int check_rows(int dtype, long long ld, int N, int V, const char *what) {
   return TL_OK;
 }
 
-// A gradient may take its logits' own place (the same rows), nothing between.
+// A gradient may take its logits' own place (the same rows), or rows that share
+// no element with them: other memory, or, with the same stride, the space
+// between them.
 int check_in_place(const void *dz, long long ldd, const LogitRows &z) {
   if (dz == z.p && (ldd == z.ld || z.N == 1)) return TL_OK;
-  const size_t es = dtype_size(z.dtype);
+  const long long es = (long long)dtype_size(z.dtype);
   const uintptr_t a = reinterpret_cast<uintptr_t>(dz), b = reinterpret_cast<uintptr_t>(z.p);
   const uintptr_t a1 = a + ((size_t)(z.N - 1) * ldd + z.V) * es, b1 = b + ((size_t)(z.N - 1) * z.ld + z.V) * es;
-  if (a < b1 && b < a1)
-    return set_error(TL_EINVAL, "dlogits overlaps logits without being the same rows");
-  return TL_OK;
+  if (a >= b1 || b >= a1) return TL_OK;
+  if (ldd == z.ld) {
+    const long long between = (a > b ? (long long)(a - b) : (long long)(b - a)) / es % ldd;
+    if (between >= z.V && between <= ldd - z.V) return TL_OK;
+  }
+  return set_error(TL_EINVAL, "dlogits overlaps logits without being the same rows");
 }
 
 }  // namespace
