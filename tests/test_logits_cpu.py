@@ -148,3 +148,15 @@ def test_binding_checks_shapes_and_types(bad, error):
     args = {k: fake(v) if isinstance(v, torch.Tensor) else v for k, v in args.items()}
     with pytest.raises(error):
         ops.token_logprobs(args.pop("logits"), args.pop("ids"), 2, 8, args.pop("logp"), **args)
+
+
+def test_stream_without_torch_s_private_call(monkeypatch):
+    """A torch that lacks the one-call form of the current stream: the public one is taken."""
+    monkeypatch.delattr(torch._C, "_cuda_getCurrentRawStream", raising=False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda idx: type("S", (), {"cuda_stream": 1234 + idx})())
+    seen = []
+    monkeypatch.setattr(ops, "_stream_set", {})
+    monkeypatch.setattr(ops, "lib", lambda: type("L", (), {"tl_set_stream": lambda self, s: seen.append(s) or 0})())
+    ops._bind_stream(1)
+    ops._bind_stream(1)
+    assert seen == [1235]

@@ -36,8 +36,17 @@ def init(device=0):
     return idx
 
 
+def _raw_stream(idx):
+    """torch's current stream of a device as a cudaStream_t: in one call where this torch has it (a call of a
+    few rows is as long as its way through Python), else by the public way."""
+    try:
+        return torch._C._cuda_getCurrentRawStream(idx)
+    except AttributeError:
+        return torch.cuda.current_stream(idx).cuda_stream
+
+
 def _bind_stream(idx):
-    s = torch._C._cuda_getCurrentRawStream(idx)   # what torch.cuda.current_stream(idx).cuda_stream reads
+    s = _raw_stream(idx)
     if _stream_set.get(idx) != s:
         check(lib().tl_set_stream(s))
         _stream_set[idx] = s
