@@ -103,3 +103,11 @@ def test_waits_that_run_out(cuda, limit_ns):
         assert out == 0
     if limit_ns <= 300:              # the barrier itself waits for a microsecond or two before it is looked at again
         assert out > 0
+
+
+@pytest.mark.parametrize("text", ["", "soon", "-5"])
+def test_a_limit_that_is_none_is_not_taken(cuda, text):
+    env = dict(os.environ, TL_COPY_TIMEOUT_NS=text)
+    r = subprocess.run([sys.executable, "-c", CODE], cwd=ROOT, capture_output=True, text=True, timeout=300, env=env)
+    assert r.returncode == 0, r.stderr[-2000:]
+    assert r.stdout.split("ended")[1].split() == ["36", "0"]

@@ -1,5 +1,6 @@
 // tl_runtime.cu -- device contexts, streams, memory and errors of libtinylm_cuda.
 #include <cstdarg>
+#include <cstdlib>
 #include <cstring>
 #include "tl_common.cuh"
 
@@ -78,8 +79,9 @@ TL_API int tl_init(int device) {
   c.gemm_ws_floats = kGemmWorkspaceFloats;
   TL_TRY_CUDA(cudaMalloc(&c.gemm_amax, sizeof(unsigned) * 8));
   if (const char *e = getenv("TL_COPY_TIMEOUT_NS")) {
-    const long long ns = atoll(e);
-    if (ns >= 0 && ns < (long long)c.copy_wait_ns) c.copy_wait_ns = (unsigned)ns;
+    char *end = nullptr;
+    const long long ns = strtoll(e, &end, 10);
+    if (end != e && !*end && ns >= 0 && ns < (long long)c.copy_wait_ns) c.copy_wait_ns = (unsigned)ns;
   }
   TL_TRY_CUDA(cudaDeviceSynchronize());
   c.ready = true;
