@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(TH + 64, TOP ? min_blocks(TH + 64) : 65536 / (
   __shared__ Part s_part[2][W];
   __shared__ float s_thr[2], s_w[2][W];
   __shared__ unsigned short s_list[TOP ? W : 1][LIST];
-  __shared__ unsigned s_count[2];
+  __shared__ unsigned s_count[3];    // the last of nobody
   __shared__ uint64_t s_full[MAX_STAGES], s_free[MAX_STAGES], s_done[2], s_taken[2];
   __shared__ int s_abort;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -627,6 +627,8 @@ __global__ void __launch_bounds__(TH + 64, TOP ? min_blocks(TH + 64) : 65536 / (
     // this row's places in shared memory: the results' warp has taken the row before last from them
     const bool mine = count_rows < 2 || pipe.wait_all(&s_taken[flip], ((count_rows >> 1) - 1) & 1);
     bool ok = mine;                  // of each lane
+    const int slot = mine ? flip : 2;              // else the row's places may still be another's
+    const unsigned cap = mine ? a.cap : 0;
     const Chunks<T> r = t.row(n);
     uint2 *keys = s_keys + flip * a.cap;
     Running run;
@@ -650,13 +652,9 @@ __global__ void __launch_bounds__(TH + 64, TOP ? min_blocks(TH + 64) : 65536 / (
       const uint32_t st = tc::smem_u32(pipe.stage(turn.s));
       bool equal = false;
       auto flush = [&] {
-        if (!mine) {                 // the row's places may still be another's
-          pass.n = 0;
-          return;
-        }
         pass.elements<T>(reinterpret_cast<const T *>(pipe.stage(turn.s)), thr, equal, [&](float f, int v) {
-          const unsigned at = atomicAdd(&s_count[flip], 1u);
-          if (at < (unsigned)a.cap) keys[at] = make_uint2(__float_as_uint(f), (unsigned)(r.first(c0) + v));
+          const unsigned at = atomicAdd(&s_count[slot], 1u);
+          if (at < cap) keys[at] = make_uint2(__float_as_uint(f), (unsigned)(r.first(c0) + v));
         });
       };
       ok &= pipe.wait(&s_full[turn.s], turn.phase);
