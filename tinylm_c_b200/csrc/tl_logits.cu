@@ -15,7 +15,9 @@
 namespace tl {
 
 // The choices below, each with what it was measured against (B200, us; "scaled"
-// is 16384 x 8192 fp32, "50k" 4096 x 50000 bf16, "131k" N x 131072 bf16):
+// is 16384 x 8192 fp32, "50k" 2047 x 50001 fp16 or 4096 x 50000 bf16, "131k" N x
+// 131072 bf16).  Both sides of a choice are of one build; figures of this build
+// stand first where it is another.
 //
 //  * A row longer than one piece of 2048 chunks is split over a cluster where
 //    there are no more rows than SMs: 131k scores with K = 20 take 8 instead of
@@ -23,19 +25,26 @@ namespace tl {
 //    against 35 for 296.  So many blocks a row that they fill the SMs once, two
 //    at least: 74 rows of 32768 fp32 take 5.6, 5.9 and 7.7 us with 2, 4 and 8.
 //    A row of one piece gains nothing from it (6.9 against 6.2 us for a
-//    distilled row of 8192 fp32).
+//    distilled row of 8192 fp32, 7.3 now).
 //  * Alternatives: pieces of 2048 chunks, one stage, 128 threads (5 blocks an
-//    SM): scaled K = 64 takes 205 us, with two stages (3 blocks) 235, with 256
-//    threads 272, with pieces of 1024 chunks 250.  Above K = 64 four warps'
-//    maxima are too few for a threshold: K = 128 takes 510 us with 256 threads
-//    and 2069 with 128.
-//  * No alternatives: pieces of 1024 chunks, two stages, 128 threads: 86 us
-//    scaled and 81 for 50k; one stage of 2048 and 256 threads 92 and 100.
-//  * Distillation: 256 threads, pieces of 2048 chunks, two stages: 219 us scaled
-//    with a tail and 105 for 2048 x 50000 fp16 (two stages against one, before
-//    the loss was added up in double: 207 against 224 and 104 against 123).  Rows
-//    of six pieces or more, which come twice, three stages: so two blocks an SM,
-//    whose rows stay in L2 in between, 218 us for 2048 rows of 131k against 242.
+//    SM): scaled K = 64 takes 211 us; 205, with two stages (3 blocks) 235, with
+//    256 threads 272, with pieces of 1024 chunks 250.  Above K = 64 rows of more
+//    than 1024 chunks have 256 threads: K = 128 takes 510 us with them and 2069
+//    with 128, whose four warps' maxima are too few for a threshold.  Rows of up
+//    to 1024 chunks keep 128 threads at any K, and there it is not always high
+//    enough: K above 124 takes all 32 maxima of each warp, and 50 to 90 % of
+//    random rows of 800 to 8192 logits overflow their list and go to select_row;
+//    16-bit rows of 32 to 127 chunks have no threshold where K is above 32 a full
+//    warp, and overflow with more logits than the list holds (320, above K = 64
+//    512).  Below that one warp sorts 2 K and more a row: 16384 x 1000 fp32, K =
+//    100 takes 271 us, 20 without alternatives.
+//  * No alternatives: pieces of 1024 chunks, two stages, 128 threads: 83 us
+//    scaled; 86 and for 50k 81, one stage of 2048 and 256 threads 92 and 100.
+//  * Distillation: 256 threads, pieces of 2048 chunks, two stages: 223 us scaled
+//    and 111 for 50k; two stages against one, in an earlier build, 207 against
+//    224 and 104 against 123.  Rows of six pieces or more, which come twice, three
+//    stages: so two blocks an SM, whose rows stay in L2 in between, 221 us for
+//    2048 rows of 131k; 218 against 242.
 //  * Short rows, up to 256 chunks, have one computing warp, if its 32 maxima are
 //    enough for a threshold (K <= 16).
 RowPlan plan_rows(const DeviceCtx *c, const LogitRows &z, int K, bool twice) {

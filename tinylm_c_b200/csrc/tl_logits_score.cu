@@ -6,12 +6,13 @@
 // largest of its 32 lanes' maxima; the threshold is the g-th largest of these,
 // g = K / j rounded up: every one of g warps has j elements at or above it.
 // j = K / F where that is 8 or more, else 5/4 of it, so that g < F: the least
-// of many maxima can be very low.  Of random logits 1.7 to 2.2 K pass.  (A
-// cluster's blocks take g in proportion to their full warps, and the least of
-// their thresholds.)  The elements that pass are collected in shared memory
-// and sorted as 64-bit keys: logit, then the lower index.  Where more pass than
-// the memory holds (many equal logits, rows in order) the K-th largest is
-// searched, counting over the row, and the lowest indices of equal ones taken.
+// of many maxima can be very low.  Of random logits 1.7 to 2.2 K pass where j
+// stays below 32; plan_rows says where it does not.  (A cluster's blocks take g
+// in proportion to their full warps, and the least of their thresholds.)  The
+// elements that pass are collected in shared memory and sorted as 64-bit keys:
+// logit, then the lower index.  Where more pass than the memory holds (many
+// equal logits, rows in order) the K-th largest is searched, counting over the
+// row, and the lowest indices of equal ones taken.
 #include <algorithm>
 #include <cmath>
 #include "tl_logits_dev.cuh"
@@ -482,7 +483,7 @@ __device__ __noinline__ void select_row(const T *row, int V, int K, float thr, u
 
 // Without alternatives 56 registers a thread: six blocks of 192 an SM instead of
 // five (16384 x 2048 bf16 21.9 against 24.8 us, 2047 x 50001 fp16 44.6 against
-// 46.2, 16384 x 8192 fp32 89 against 90).
+// 46.2).
 template <typename T, int TH, bool ENT, bool TOP>
 __global__ void __launch_bounds__(TH + 64, TOP ? min_blocks(TH + 64) : 65536 / (56 * (TH + 64))) score_kernel(const ScoreArgs a) {
   constexpr int W = TH / 32;
